@@ -353,6 +353,34 @@ int smlm_b200_rms_norm_bwd(void* dx, void* dw, const void* go, const void* x, co
                            void* workspace, size_t workspace_bytes, int rows, int cols, int dtype, int dw_fp32,
                            void* stream);
 
+/* ---- norms of queries and keys per head, with the rotary embedding: rows that are trained ------------- */
+
+/* For q [T, num_qo_heads, head_dim] and k [T, num_kv_heads, head_dim], head_dim 128, rows q_stride / k_stride elements apart
+ * (multiples of 8, at least a row: slices of one projection are taken as they lie), per row and head:
+ *   n = x * rsqrt(mean(x^2) + eps) * w            (wq and wk [head_dim]; both NULL: n = x)
+ *   y = n rotated for positions[t], Llama convention with base rope_theta   (positions NULL: y = n)
+ * in fp32, rounded once to the 16-bit `dtype`; yq and yk contiguous.  Weights, positions or both.  positions: int32, or int64
+ * where positions_64 is set, below 2^24 in absolute value; the angles are formed to 2^-40 turns, so that far positions
+ * lose nothing.  No workspace. */
+int smlm_b200_qk_norm_rope(void* yq, void* yk, const void* q, const void* k, const void* wq, const void* wk,
+                           const void* positions, long long q_stride, long long k_stride, int T, int num_qo_heads,
+                           int num_kv_heads, int head_dim, int positions_64, double rope_theta, float eps, int dtype,
+                           void* stream);
+
+/* Bytes of the workspace of smlm_b200_qk_norm_rope_bwd (fp32 shares of dwq and dwk, one row per CTA; needs no
+ * initialisation; not used without weights). */
+size_t smlm_b200_qk_norm_rope_bwd_workspace_bytes(int T, int num_qo_heads, int num_kv_heads);
+
+/* Backward of the above from the gradients gq and gk of yq and yk (contiguous):
+ *   dn = g rotated back      dw = sum over rows and heads of x s dn      dx = s (w dn - x s^2 mean(w dn x)),  s the rsqrt
+ * dq and dk contiguous; dwq and dwk [head_dim] in `dtype` (NULL without weights), summed in fp32 in a fixed order.  T must be
+ * positive. */
+int smlm_b200_qk_norm_rope_bwd(void* dq, void* dk, void* dwq, void* dwk, const void* gq, const void* gk, const void* q,
+                               const void* k, const void* wq, const void* wk, const void* positions, void* workspace,
+                               size_t workspace_bytes, long long q_stride, long long k_stride, int T, int num_qo_heads,
+                               int num_kv_heads, int head_dim, int positions_64, double rope_theta, float eps, int dtype,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -98,6 +98,50 @@ int smlm_b200_init_kv(const void* const* kv_ptrs, const int32_t* kv_indptr, cons
                       int total_pages, int total_tokens, int num_layers, int layer_idx, int num_kv_heads, int head_dim,
                       int page_size, int dtype, void* stream);
 
+/* ---- operators around a cache that several continuations share -------------------------------------- */
+
+/* Bytes of the workspace of smlm_b200_batch_extend for a batch of these sizes (0: none is needed).  Its contents
+ * matter neither before nor after a call; launches that may overlap in time must not share one. */
+size_t smlm_b200_batch_extend_workspace_bytes(int batch_size, int total_q, int total_pages, int page_size,
+                                              int num_qo_heads, int num_kv_heads);
+
+/* Attention of a chunk of new tokens per request over its paged cache, which already holds them (init_kv or
+ * norm_append_kv ran before).  Request b owns the rows qo_indptr[b] .. qo_indptr[b + 1] of q and o ([total_q, num_qo_heads,
+ * head_dim], 16-byte aligned), n_b >= 0 of them; its query i stands at position L_b - n_b + i and sees the keys up to its own:
+ *   o[i, h] = softmax( rope(q[i, h], pos_i) . rope(K_b[0..pos_i, h / group])^T / sqrt(head_dim) ) . V_b[0..pos_i]
+ * What smlm_b200_batch_prefill computes, for chunks that are short against their cache: the pages are read in place, and
+ * long caches are cut into ranges of keys so that a few new tokens fill the machine.  The ranges follow from the lengths
+ * on the device alone: the same batch gives the same result, whatever its page table's length.  Rows of no request are left
+ * as they were; a row that sees no key is zeros.  Status word: bit 1 also where a request has more queries than keys. */
+int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, const void* const* kv_ptrs,
+                           const int32_t* kv_indptr, const int32_t* last_page_offset, void* workspace,
+                           size_t workspace_bytes, int* status_word, int batch_size, int total_q, int total_pages,
+                           int num_qo_heads, int num_kv_heads, int head_dim, int num_layers, int layer_idx, int page_size,
+                           double rope_theta, int dtype, void* stream);
+
+/* The new tokens' way into the cache for models that normalise queries and keys per head:
+ *   yq[t, h]  = q[t, h] * rsqrt(mean(q[t, h]^2) + eps) * wq         [total_tokens, num_qo_heads, head_dim], contiguous
+ *   the pages receive k[t, h] normalised likewise with wk, not rotated, and v[t, h] as it is
+ * Which entries they go to is smlm_b200_init_kv's rule (seqlen_indptr[batch + 1] given: the last entries of each cache) or
+ * smlm_b200_append_kv's (seqlen_indptr NULL: one token per request, total_tokens == batch_size).  q, k and v may be slices of one
+ * projection: rows are q_stride / k_stride / v_stride elements apart (multiples of 8, at least a row), heads head_dim
+ * apart.  wq and wk [head_dim] in `dtype`; the norm is formed in fp32 and rounded once.  A token whose place the pages do not
+ * hold sets bit 1 of the status word and is not written; its query still is.  Rows of no request are left as they were. */
+int smlm_b200_norm_append_kv(void* yq, const void* q, const void* k, const void* v, const void* wq, const void* wk,
+                             const void* const* kv_ptrs, const int32_t* kv_indptr, const int32_t* last_page_offset,
+                             const int32_t* seqlen_indptr, int* status_word, long long q_stride, long long k_stride,
+                             long long v_stride, int batch_size, int total_tokens, int total_pages, int num_qo_heads,
+                             int num_kv_heads, int head_dim, int num_layers, int layer_idx, int page_size, float eps,
+                             int dtype, void* stream);
+
+/* Copies n pages: page src_ptrs[i] to page dst_ptrs[i], all layers and heads, the first entries[i] positions of each (NULL:
+ * whole pages); the other positions of the destination stay as they are.  A page may be the source of several copies; no
+ * page may be the destination of two, nor source and destination at once.  Null or misaligned addresses (bit 2 of the
+ * status word) and entries outside 0 .. page_size (bit 1) are skipped. */
+int smlm_b200_copy_pages(const void* const* dst_ptrs, const void* const* src_ptrs, const int32_t* entries,
+                         int* status_word, int n, int num_layers, int num_kv_heads, int head_dim, int page_size, int dtype,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

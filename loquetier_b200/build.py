@@ -3,7 +3,7 @@
     python -m loquetier_b200.build [--force] [--verbose]
 
 The product is ``loquetier_b200/libsmlm_b200.so``: a plain C-ABI shared library
-(declared in ``include/smlm_b200.h``) with no dependency on torch or Python."""
+(declared in ``include/smlm_b200.h`` and ``smlm_b200_kv.h``) with no dependency on torch or Python."""
 from __future__ import annotations
 
 import os
@@ -13,10 +13,10 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsmlm_b200.so")
-SOURCES = [os.path.join(CSRC, "smlm_capi.cu")]
+SOURCES = [os.path.join(CSRC, f) for f in ("smlm_capi.cu", "cache_capi.cu")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--use_fast_math", "-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v",
+    "--use_fast_math", "-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v", "--threads", "2",
 ]
 
 

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_longlong, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsmlm_b200.so")
@@ -76,6 +76,14 @@ SIGNATURES = {
     "smlm_b200_batch_decode": (c_int, [c_void_p] * 6 + [c_size_t, c_void_p] + [c_int] * 8 + [c_float, c_int, c_void_p]),
     "smlm_b200_append_kv": (c_int, [c_void_p] * 6 + [c_int] * 8 + [c_void_p]),
     "smlm_b200_init_kv": (c_int, [c_void_p] * 7 + [c_int] * 9 + [c_void_p]),
+    "smlm_b200_batch_extend_workspace_bytes": (c_size_t, [c_int] * 6),
+    "smlm_b200_batch_extend": (c_int, [c_void_p] * 7 + [c_size_t, c_void_p] + [c_int] * 9 + [c_double, c_int, c_void_p]),
+    "smlm_b200_norm_append_kv": (c_int, [c_void_p] * 11 + [c_longlong] * 3 + [c_int] * 9 + [c_float, c_int, c_void_p]),
+    "smlm_b200_copy_pages": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
+    "smlm_b200_qk_norm_rope": (c_int, [c_void_p] * 7 + [c_longlong] * 2 + [c_int] * 5 + [c_double, c_float, c_int, c_void_p]),
+    "smlm_b200_qk_norm_rope_bwd_workspace_bytes": (c_size_t, [c_int] * 3),
+    "smlm_b200_qk_norm_rope_bwd": (c_int, [c_void_p] * 12 + [c_size_t] + [c_longlong] * 2 + [c_int] * 5
+                                   + [c_double, c_float, c_int, c_void_p]),
     "smlm_b200_rms_norm": (c_int, [c_void_p] * 4 + [c_int, c_int, c_float, c_int, c_void_p]),
     "smlm_b200_rms_norm_bwd_workspace_bytes": (c_size_t, [c_int, c_int]),
     "smlm_b200_rms_norm_bwd": (c_int, [c_void_p] * 7 + [c_size_t] + [c_int] * 4 + [c_void_p]),

@@ -1,0 +1,279 @@
+// C ABI of the operators around a cache that several continuations share: attention of a chunk of new tokens, norms of
+// queries and keys per head, page copies.  Declarations: include/smlm_b200_kv.h, include/smlm_b200.h.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/smlm_b200.h"
+#include "../../include/smlm_b200_kv.h"
+#include "head_norm.cuh"
+#include "kv_pages.cuh"
+#include "paged_extend.cuh"
+#include "smlm_launch.cuh"
+
+namespace {
+
+// base^(-2 i / 128) / pi as pairs of floats; the last base's table is kept per thread (64 powers take a microsecond)
+const RotTable& rot_table(double base) {
+  thread_local RotTable table;
+  thread_local double of = 0.0;
+  if (of != base) {
+    for (int i = 0; i < 64; ++i) {
+      const double f = std::pow(base, -i / 64.0) / 3.14159265358979323846;
+      table.hi[i] = static_cast<float>(f);
+      table.lo[i] = static_cast<float>(f - static_cast<double>(table.hi[i]));
+    }
+    of = base;
+  }
+  return table;
+}
+
+// How an extend launch is laid out: everything follows from sizes the host knows, so that the workspace query and the launch agree.
+struct ExPlan {
+  int nt;          // column tiles of eight rows per row tile
+  int rows;        // rows of a tile
+  int target;      // ranges aimed at per kv head
+  int min_tiles;   // key tiles of a range at least
+  int slots;       // (tile, range) pairs per kv head
+  bool merge;      // a tile may have several ranges
+  size_t bytes;    // of parked states
+};
+
+ExPlan extend_plan(int batch, int total_q, int total_pages, int page_size, int num_kv_heads, int group) {
+  ExPlan p;
+  const long long all_rows = static_cast<long long>(total_q) * group;
+  const long long mean = (all_rows + batch - 1) / batch;
+  p.nt = mean <= 8 ? 1 : mean <= 16 ? 2 : 4;
+  p.rows = ex_rows(p.nt);
+  p.min_tiles = kPdWarps;
+  const long long key_tiles = static_cast<long long>(total_pages) * page_size / kPdTile + 1;
+  const long long tiles = all_rows / p.rows + batch;
+  const long long most = (all_rows / p.rows + 1) * key_tiles / p.min_tiles + 1;
+  const long long want = std::max(1, 2 * kNumSMs * ex_ctas_per_sm(p.nt) / num_kv_heads);
+  p.target = static_cast<int>(std::min(want, most));
+  p.slots = static_cast<int>(std::min<long long>(tiles + p.target, 0x7fffffffLL / num_kv_heads));
+  p.merge = key_tiles > p.min_tiles;
+  p.bytes = p.merge ? static_cast<size_t>(p.slots) * num_kv_heads * p.rows * kPdRec * sizeof(float) : 0;
+  return p;
+}
+
+template <typename T, int NT>
+int launch_extend(const ExArgs& a, const ExPlan& p, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.slots) * a.num_kv_heads, 1, 1);
+  const int rc = launch(paged_extend_kernel<T, NT>, grid, kExThreads, 1, ex_smem(NT), stream, a);
+  if (rc != SMLM_OK || !p.merge) return rc;
+  return launch(paged_extend_merge_kernel<T, 8 * NT, kPdTile>, grid, kExThreads, 1, 0, stream, a);
+}
+
+template <typename T>
+int dispatch_extend(const ExArgs& a, const ExPlan& p, cudaStream_t stream) {
+  switch (p.nt) {
+    case 1: return launch_extend<T, 1>(a, p, stream);
+    case 2: return launch_extend<T, 2>(a, p, stream);
+    default: return launch_extend<T, 4>(a, p, stream);
+  }
+}
+
+// warps that share a token's heads: few tokens are spread over the machine, four heads per warp at least
+inline int head_splits(int T, int heads) {
+  const int want = (8 * kNumSMs * 2 + T - 1) / std::max(T, 1);
+  return std::max(1, std::min(want, (heads + 3) / 4));
+}
+
+template <typename T>
+int launch_qk_fwd(const HeadNormArgs& a, cudaStream_t stream) {
+  const bool norm = a.wq != nullptr, rope = a.positions != nullptr;
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.T) * a.splits + kHnWarps - 1) / kHnWarps), 1, 1);
+  if (norm) return rope ? launch(qk_norm_rope_kernel<T, true, true>, grid, kHnThreads, 1, 0, stream, a)
+                        : launch(qk_norm_rope_kernel<T, true, false>, grid, kHnThreads, 1, 0, stream, a);
+  return launch(qk_norm_rope_kernel<T, false, true>, grid, kHnThreads, 1, 0, stream, a);
+}
+
+inline int qk_bwd_grid(int T, int splits) {
+  const long long ctas = (static_cast<long long>(T) * splits + kHnWarps - 1) / kHnWarps;
+  return static_cast<int>(std::min<long long>(ctas, 2 * kNumSMs));
+}
+
+template <typename T>
+int launch_qk_bwd(const HeadNormArgs& a, void* dwq, void* dwk, cudaStream_t stream) {
+  const bool norm = a.wq != nullptr, rope = a.positions != nullptr;
+  const dim3 grid(qk_bwd_grid(a.T, a.splits), 1, 1);
+  if (!norm) return launch(qk_norm_rope_bwd_kernel<T, false, true>, grid, kHnThreads, 1, 0, stream, a);
+  const int rc = rope ? launch(qk_norm_rope_bwd_kernel<T, true, true>, grid, kHnThreads, 1, 0, stream, a)
+                      : launch(qk_norm_rope_bwd_kernel<T, true, false>, grid, kHnThreads, 1, 0, stream, a);
+  if (rc != SMLM_OK) return rc;
+  return launch(head_norm_dw_kernel<T>, dim3(2 * kPdDim / 8, 1, 1), 256, 1, 0, stream, dwq, dwk, a.partial,
+                static_cast<int>(grid.x));
+}
+
+// the checks that both directions share; rows that are strided have to keep the 16-byte alignment of every head
+int qk_check(const void* q, const void* k, const void* wq, const void* wk, const void* positions, long long q_stride,
+             long long k_stride, int T, int Nq, int Nk, int head_dim, int positions_64, double rope_theta, int dtype) {
+  (void)positions_64;
+  if (T < 0 || Nq <= 0 || Nk <= 0 || (wq == nullptr) != (wk == nullptr) || (wq == nullptr && positions == nullptr) ||
+      (positions != nullptr && !(rope_theta > 0.0)))
+    return SMLM_ERR_INVALID_ARGUMENT;
+  if (dtype != SMLM_F16 && dtype != SMLM_BF16) return SMLM_ERR_DTYPE;
+  if (head_dim != kPdDim) return SMLM_ERR_NO_KERNEL;
+  if (T == 0) return SMLM_OK;
+  if (q == nullptr || k == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
+  if (q_stride < static_cast<long long>(Nq) * kPdDim || k_stride < static_cast<long long>(Nk) * kPdDim)
+    return SMLM_ERR_INVALID_ARGUMENT;   // rows that overlap
+  if (!aligned16(q) || !aligned16(k) || !aligned16(wq) || !aligned16(wk) || q_stride % 8 != 0 || k_stride % 8 != 0)
+    return SMLM_ERR_MISALIGNED;
+  return SMLM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t smlm_b200_batch_extend_workspace_bytes(int batch_size, int total_q, int total_pages, int page_size,
+                                              int num_qo_heads, int num_kv_heads) {
+  if (batch_size <= 0 || total_q <= 0 || total_pages < 0 || page_size <= 0 || num_kv_heads <= 0 ||
+      num_qo_heads < num_kv_heads)
+    return 0;
+  return extend_plan(batch_size, total_q, total_pages, page_size, num_kv_heads, num_qo_heads / num_kv_heads).bytes;
+}
+
+int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, const void* const* kv_ptrs,
+                           const int32_t* kv_indptr, const int32_t* last_page_offset, void* workspace,
+                           size_t workspace_bytes, int* status_word, int batch_size, int total_q, int total_pages,
+                           int num_qo_heads, int num_kv_heads, int head_dim, int num_layers, int layer_idx, int page_size,
+                           double rope_theta, int dtype, void* stream) {
+  if (batch_size < 0 || total_q < 0 || total_pages < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || num_layers <= 0 ||
+      layer_idx < 0 || layer_idx >= num_layers || !(rope_theta > 0.0))
+    return SMLM_ERR_INVALID_ARGUMENT;
+  if (dtype != SMLM_F16 && dtype != SMLM_BF16) return SMLM_ERR_DTYPE;
+  if (num_qo_heads % num_kv_heads != 0 || !kv_shape_ok(head_dim, page_size)) return SMLM_ERR_NO_KERNEL;
+  const int group = num_qo_heads / num_kv_heads;
+  if (group != 1 && group != 2 && group != 4 && group != 8) return SMLM_ERR_NO_KERNEL;
+  if (batch_size == 0 || total_q == 0) return SMLM_OK;
+  if (o == nullptr || q == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || last_page_offset == nullptr ||
+      (kv_ptrs == nullptr && total_pages > 0))
+    return SMLM_ERR_INVALID_ARGUMENT;
+  if (!aligned16(o) || !aligned16(q)) return SMLM_ERR_MISALIGNED;
+  if (static_cast<long long>(total_q) * num_qo_heads > 0x7fffffffLL ||
+      static_cast<long long>(total_pages) * page_size > 0x7fffffffLL)
+    return SMLM_ERR_INVALID_ARGUMENT;
+  const ExPlan p = extend_plan(batch_size, total_q, total_pages, page_size, num_kv_heads, group);
+  if (p.bytes > 0) {
+    if (workspace == nullptr || workspace_bytes < p.bytes) return SMLM_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return SMLM_ERR_MISALIGNED;
+  }
+  ExArgs a;
+  a.o = o; a.q = q; a.qo_indptr = qo_indptr; a.kv_ptrs = kv_ptrs; a.kv_indptr = kv_indptr;
+  a.last_page_offset = last_page_offset; a.partial = static_cast<float*>(workspace); a.err = status_word;
+  a.batch = batch_size; a.total_q = total_q; a.total_pages = total_pages; a.num_kv_heads = num_kv_heads;
+  a.num_layers = num_layers; a.layer_idx = layer_idx; a.page_size = page_size;
+  a.lg = group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3;
+  a.target = p.target; a.min_tiles = p.min_tiles; a.slots = p.slots;
+  a.rot = rot_table(rope_theta);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == SMLM_F16 ? dispatch_extend<__half>(a, p, st) : dispatch_extend<__nv_bfloat16>(a, p, st);
+}
+
+int smlm_b200_copy_pages(const void* const* dst_ptrs, const void* const* src_ptrs, const int32_t* entries,
+                         int* status_word, int n, int num_layers, int num_kv_heads, int head_dim, int page_size, int dtype,
+                         void* stream) {
+  if (n < 0 || num_layers <= 0 || num_kv_heads <= 0) return SMLM_ERR_INVALID_ARGUMENT;
+  if (dtype != SMLM_F16 && dtype != SMLM_BF16) return SMLM_ERR_DTYPE;
+  if (!kv_shape_ok(head_dim, page_size)) return SMLM_ERR_NO_KERNEL;
+  if (n == 0) return SMLM_OK;
+  if (dst_ptrs == nullptr || src_ptrs == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
+  const long long chunks = static_cast<long long>(num_layers) * 2 * num_kv_heads * page_size * 16;
+  if (chunks > 0x7fffffffLL) return SMLM_ERR_INVALID_ARGUMENT;   // a page of 32 GB
+  CopyPagesArgs a;
+  a.dst = dst_ptrs; a.src = src_ptrs; a.entries = entries; a.err = status_word;
+  a.n = n; a.runs = num_layers * 2 * num_kv_heads; a.page_size = page_size;
+  const dim3 grid(static_cast<unsigned>((chunks + kCpChunks - 1) / kCpChunks), std::min(n, 65535), 1);
+  return launch(copy_pages_kernel, grid, kCpThreads, 1, 0, static_cast<cudaStream_t>(stream), a);
+}
+
+int smlm_b200_norm_append_kv(void* yq, const void* q, const void* k, const void* v, const void* wq, const void* wk,
+                             const void* const* kv_ptrs, const int32_t* kv_indptr, const int32_t* last_page_offset,
+                             const int32_t* seqlen_indptr, int* status_word, long long q_stride, long long k_stride,
+                             long long v_stride, int batch_size, int total_tokens, int total_pages, int num_qo_heads,
+                             int num_kv_heads, int head_dim, int num_layers, int layer_idx, int page_size, float eps,
+                             int dtype, void* stream) {
+  if (batch_size < 0 || total_tokens < 0 || total_pages < 0 || num_layers <= 0 || layer_idx < 0 ||
+      layer_idx >= num_layers || (seqlen_indptr == nullptr && total_tokens != batch_size) || wq == nullptr || wk == nullptr)
+    return SMLM_ERR_INVALID_ARGUMENT;
+  const int rc = qk_check(q, k, wq, wk, nullptr, q_stride, k_stride, total_tokens, num_qo_heads, num_kv_heads, head_dim, 0,
+                          1.0, dtype);
+  if (rc != SMLM_OK) return rc;
+  if (!kv_shape_ok(head_dim, page_size)) return SMLM_ERR_NO_KERNEL;
+  if (batch_size == 0 || total_tokens == 0) return SMLM_OK;
+  if (yq == nullptr || v == nullptr || kv_indptr == nullptr || last_page_offset == nullptr ||
+      (kv_ptrs == nullptr && total_pages > 0) || v_stride < static_cast<long long>(num_kv_heads) * kPdDim)
+    return SMLM_ERR_INVALID_ARGUMENT;
+  if (!aligned16(yq) || !aligned16(v) || v_stride % 8 != 0) return SMLM_ERR_MISALIGNED;
+  NormAppendArgs a;
+  a.q = q; a.k = k; a.v = v; a.wq = wq; a.wk = wk; a.yq = yq; a.kv_ptrs = kv_ptrs; a.kv_indptr = kv_indptr;
+  a.last_page_offset = last_page_offset; a.append_indptr = seqlen_indptr; a.err = status_word;
+  a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+  a.T = total_tokens; a.batch = batch_size; a.Nq = num_qo_heads; a.Nk = num_kv_heads; a.num_layers = num_layers;
+  a.layer_idx = layer_idx; a.page_size = page_size; a.total_pages = total_pages; a.eps = eps;
+  a.splits = head_splits(total_tokens, std::max(num_qo_heads, num_kv_heads));
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.T) * a.splits + kHnWarps - 1) / kHnWarps), 1, 1);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == SMLM_F16 ? launch(norm_append_kernel<__half>, grid, kHnThreads, 1, 0, st, a)
+                           : launch(norm_append_kernel<__nv_bfloat16>, grid, kHnThreads, 1, 0, st, a);
+}
+
+int smlm_b200_qk_norm_rope(void* yq, void* yk, const void* q, const void* k, const void* wq, const void* wk,
+                           const void* positions, long long q_stride, long long k_stride, int T, int num_qo_heads,
+                           int num_kv_heads, int head_dim, int positions_64, double rope_theta, float eps, int dtype,
+                           void* stream) {
+  const int rc = qk_check(q, k, wq, wk, positions, q_stride, k_stride, T, num_qo_heads, num_kv_heads, head_dim,
+                          positions_64, rope_theta, dtype);
+  if (rc != SMLM_OK || T == 0) return rc;
+  if (yq == nullptr || yk == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
+  if (!aligned16(yq) || !aligned16(yk)) return SMLM_ERR_MISALIGNED;
+  HeadNormArgs a = {};
+  a.q = q; a.k = k; a.wq = wq; a.wk = wk; a.positions = positions; a.yq = yq; a.yk = yk;
+  a.q_stride = q_stride; a.k_stride = k_stride; a.T = T; a.Nq = num_qo_heads; a.Nk = num_kv_heads; a.pos64 = positions_64;
+  a.eps = eps;
+  a.splits = head_splits(T, std::max(num_qo_heads, num_kv_heads));
+  if (positions != nullptr) a.rot = rot_table(rope_theta);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == SMLM_F16 ? launch_qk_fwd<__half>(a, st) : launch_qk_fwd<__nv_bfloat16>(a, st);
+}
+
+size_t smlm_b200_qk_norm_rope_bwd_workspace_bytes(int T, int num_qo_heads, int num_kv_heads) {
+  if (T <= 0 || num_qo_heads <= 0 || num_kv_heads <= 0) return 0;
+  return static_cast<size_t>(qk_bwd_grid(T, head_splits(T, std::max(num_qo_heads, num_kv_heads)))) * 2 * kPdDim *
+         sizeof(float);
+}
+
+int smlm_b200_qk_norm_rope_bwd(void* dq, void* dk, void* dwq, void* dwk, const void* gq, const void* gk, const void* q,
+                               const void* k, const void* wq, const void* wk, const void* positions, void* workspace,
+                               size_t workspace_bytes, long long q_stride, long long k_stride, int T, int num_qo_heads,
+                               int num_kv_heads, int head_dim, int positions_64, double rope_theta, float eps, int dtype,
+                               void* stream) {
+  const int rc = qk_check(q, k, wq, wk, positions, q_stride, k_stride, T, num_qo_heads, num_kv_heads, head_dim,
+                          positions_64, rope_theta, dtype);
+  if (rc != SMLM_OK) return rc;
+  if (T == 0) return SMLM_ERR_INVALID_ARGUMENT;   // a sum over no rows: the caller zeroes the weight gradients itself
+  if (dq == nullptr || dk == nullptr || gq == nullptr || gk == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
+  if (!aligned16(dq) || !aligned16(dk) || !aligned16(gq) || !aligned16(gk)) return SMLM_ERR_MISALIGNED;
+  if (wq != nullptr) {
+    if (dwq == nullptr || dwk == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
+    if (workspace == nullptr ||
+        workspace_bytes < smlm_b200_qk_norm_rope_bwd_workspace_bytes(T, num_qo_heads, num_kv_heads))
+      return SMLM_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return SMLM_ERR_MISALIGNED;
+  }
+  HeadNormArgs a = {};
+  a.q = q; a.k = k; a.wq = wq; a.wk = wk; a.positions = positions; a.yq = dq; a.yk = dk; a.gq = gq; a.gk = gk;
+  a.partial = static_cast<float*>(workspace);
+  a.q_stride = q_stride; a.k_stride = k_stride; a.T = T; a.Nq = num_qo_heads; a.Nk = num_kv_heads; a.pos64 = positions_64;
+  a.eps = eps;
+  a.splits = head_splits(T, std::max(num_qo_heads, num_kv_heads));
+  if (positions != nullptr) a.rot = rot_table(rope_theta);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == SMLM_F16 ? launch_qk_bwd<__half>(a, dwq, dwk, st) : launch_qk_bwd<__nv_bfloat16>(a, dwq, dwk, st);
+}
+
+}  // extern "C"

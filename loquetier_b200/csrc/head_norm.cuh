@@ -1,0 +1,380 @@
+// Norms of queries and keys over each head's 128 dimensions, with the rotary position embedding in the same pass
+// (training rows, forward and backward) or on the way into the paged cache (served rows; the cache keeps keys
+// un-rotated).
+//
+//   s = rsqrt(mean(x^2) + eps)     n = x s w     y = R(p) n
+//   R(p): dimensions i and i + 64 turned by the angle p base^(-2 i / 128)
+//   backward:  dn = R(-p) dy     dw = sum over rows of x s dn     dx = s (w dn - x s^2 mean(w dn x))
+//
+// Everything is bound by HBM: a value is read once and written once, the norm's factor and the rotation are made in
+// registers.  Eight lanes share a head - lane c holds dimensions 8 c .. 8 c + 7 and their partners 64 dimensions on, two
+// 16-byte loads, no exchange for the rotation and three shuffles for the sum - so a warp has four heads in flight per
+// step, and a lane meets the same eight frequencies for every head of its token: their sines are made once per token.
+#pragma once
+#include "paged_kv.cuh"
+#include "rms_norm.cuh"
+#include "rotary.cuh"
+
+namespace smlm {
+
+constexpr int kHnThreads = 256;
+constexpr int kHnWarps = kHnThreads / 32;
+
+struct HeadNormArgs {
+  const void* q;            // [T, Nq, 128], rows q_stride elements apart
+  const void* k;            // [T, Nk, 128]
+  const void* wq;           // [128], null: no norm
+  const void* wk;
+  const void* positions;    // int32 or int64 [T], null: no rotation
+  void* yq;                 // [T, Nq, 128] contiguous
+  void* yk;
+  const void* gq;           // backward: gradients of yq and yk, contiguous; yq and yk then are dq and dk
+  const void* gk;
+  float* partial;           // backward: [gridDim.x][2][128] shares of dwq and dwk
+  long long q_stride, k_stride;
+  int T, Nq, Nk, pos64, splits;   // splits: warps that share a token's heads
+  float eps;
+  RotTable rot;
+};
+
+// the lane's eight cosines and sines at a token's position; freq: the table in shared memory
+template <bool ROPE>
+__device__ __forceinline__ void token_rotation(const HeadNormArgs& a, const float* freq, int t, int c, float (&cs)[8],
+                                               float (&sn)[8]) {
+  if (ROPE) {
+    const float pos = a.pos64 ? static_cast<float>(static_cast<const long long*>(a.positions)[t])
+                              : static_cast<float>(static_cast<const int*>(a.positions)[t]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rot_sincos(pos, freq[c * 8 + i], freq[64 + c * 8 + i], &sn[i], &cs[i]);
+  }
+}
+
+__device__ __forceinline__ float sum8(float v) {   // over the eight lanes of a head
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  v += __shfl_xor_sync(0xffffffffu, v, 2);
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  return v;
+}
+
+// forward of the heads first .. first + 3, then `step` further on, of one token; x and y point at the token's first head,
+// hl is the lane's head within four
+template <typename T, bool NORM, bool ROPE, int U>
+__device__ __forceinline__ void heads_forward(const T* x, T* y, int heads, int first, int step, const float (&w)[16],
+                                              const float (&cs)[8], const float (&sn)[8], int c, int hl, float eps) {
+  for (int h0 = first; h0 < heads; h0 += U * step) {   // uniform over the warp
+    uint4 lo[U], hi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + hl + u * step;
+      lo[u] = hi[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (h < heads) {
+        lo[u] = __ldg(reinterpret_cast<const uint4*>(x + h * kPdDim + c * 8));
+        hi[u] = __ldg(reinterpret_cast<const uint4*>(x + h * kPdDim + 64 + c * 8));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + hl + u * step;
+      float p[8], q[8];
+      unpack8<T>(lo[u], p);
+      unpack8<T>(hi[u], q);
+      if (NORM) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += p[i] * p[i] + q[i] * q[i];
+        const float s = rsqrtf(sum8(ss) * (1.0f / kPdDim) + eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] *= s * w[i];
+          q[i] *= s * w[8 + i];
+        }
+      }
+      if (ROPE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float r = p[i] * cs[i] - q[i] * sn[i];
+          q[i] = q[i] * cs[i] + p[i] * sn[i];
+          p[i] = r;
+        }
+      }
+      if (h < heads) {
+        *reinterpret_cast<uint4*>(y + h * kPdDim + c * 8) = pack8<T>(p);
+        *reinterpret_cast<uint4*>(y + h * kPdDim + 64 + c * 8) = pack8<T>(q);
+      }
+    }
+  }
+}
+
+// the lane's sixteen weights of a head
+template <typename T, bool NORM>
+__device__ __forceinline__ void load_weight(const void* w, int c, float (&f)[16]) {
+  if (NORM) {
+    float a[8], b[8];
+    unpack8<T>(__ldg(static_cast<const uint4*>(w) + c), a);
+    unpack8<T>(__ldg(static_cast<const uint4*>(w) + 8 + c), b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[i] = a[i];
+      f[8 + i] = b[i];
+    }
+  }
+}
+
+// One warp per (token, share of its heads).
+template <typename T, bool NORM, bool ROPE>
+__global__ void __launch_bounds__(kHnThreads) qk_norm_rope_kernel(const __grid_constant__ HeadNormArgs a) {
+  __shared__ __align__(16) float freq[ROPE ? 128 : 4];
+  const int lane = threadIdx.x & 31, c = lane & 7, hl = lane >> 3;
+  if (ROPE) {
+    load_rot_table(a.rot, freq);
+    __syncthreads();
+  }
+  pdl_wait();
+  pdl_trigger();
+  const long long unit = static_cast<long long>(blockIdx.x) * kHnWarps + (threadIdx.x >> 5);
+  const int t = static_cast<int>(unit / a.splits), sp = static_cast<int>(unit % a.splits);
+  if (t >= a.T) return;
+  float wq[16], wk[16], cs[8], sn[8];
+  load_weight<T, NORM>(a.wq, c, wq);
+  load_weight<T, NORM>(a.wk, c, wk);
+  token_rotation<ROPE>(a, freq, t, c, cs, sn);
+  const int first = sp * 4, step = 4 * a.splits;
+  heads_forward<T, NORM, ROPE, 2>(static_cast<const T*>(a.q) + t * a.q_stride,
+                                  static_cast<T*>(a.yq) + static_cast<size_t>(t) * a.Nq * kPdDim, a.Nq, first, step, wq, cs,
+                                  sn, c, hl, a.eps);
+  heads_forward<T, NORM, ROPE, 2>(static_cast<const T*>(a.k) + t * a.k_stride,
+                                  static_cast<T*>(a.yk) + static_cast<size_t>(t) * a.Nk * kPdDim, a.Nk, first, step, wk, cs,
+                                  sn, c, hl, a.eps);
+}
+
+template <typename T, bool NORM, bool ROPE>
+__device__ __forceinline__ void heads_backward(const T* x, const T* g, T* dx, int heads, int first, int step,
+                                               const float (&w)[16], float (&dw)[16], const float (&cs)[8],
+                                               const float (&sn)[8], int c, int hl, float eps) {
+  for (int h0 = first; h0 < heads; h0 += step) {   // uniform over the warp
+    const int h = h0 + hl;
+    uint4 xl = make_uint4(0u, 0u, 0u, 0u), xh = xl, gl = xl, gh = xl;
+    if (h < heads) {
+      gl = __ldg(reinterpret_cast<const uint4*>(g + h * kPdDim + c * 8));
+      gh = __ldg(reinterpret_cast<const uint4*>(g + h * kPdDim + 64 + c * 8));
+      if (NORM) {
+        xl = __ldg(reinterpret_cast<const uint4*>(x + h * kPdDim + c * 8));
+        xh = __ldg(reinterpret_cast<const uint4*>(x + h * kPdDim + 64 + c * 8));
+      }
+    }
+    float dp[8], dq[8];   // the gradient in front of the rotation
+    unpack8<T>(gl, dp);
+    unpack8<T>(gh, dq);
+    if (ROPE) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float r = dp[i] * cs[i] + dq[i] * sn[i];
+        dq[i] = dq[i] * cs[i] - dp[i] * sn[i];
+        dp[i] = r;
+      }
+    }
+    if (NORM) {
+      float p[8], q[8];
+      unpack8<T>(xl, p);
+      unpack8<T>(xh, q);
+      float ss = 0.f, dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ss += p[i] * p[i] + q[i] * q[i];
+        dot += w[i] * dp[i] * p[i] + w[8 + i] * dq[i] * q[i];
+      }
+      const float s = rsqrtf(sum8(ss) * (1.0f / kPdDim) + eps);
+      const float coef = sum8(dot) * s * s * (1.0f / kPdDim);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dw[i] += p[i] * s * dp[i];
+        dw[8 + i] += q[i] * s * dq[i];
+        dp[i] = s * (w[i] * dp[i] - p[i] * coef);
+        dq[i] = s * (w[8 + i] * dq[i] - q[i] * coef);
+      }
+    }
+    if (h < heads) {
+      *reinterpret_cast<uint4*>(dx + h * kPdDim + c * 8) = pack8<T>(dp);
+      *reinterpret_cast<uint4*>(dx + h * kPdDim + 64 + c * 8) = pack8<T>(dq);
+    }
+  }
+}
+
+// Warps walk over (token, share of its heads) with a fixed stride and keep their share of dw in fp32 registers; the CTA
+// adds its warps' in warp order and parks one row, which head_norm_dw_kernel adds in row order: the same result each time.
+template <typename T, bool NORM, bool ROPE>
+__global__ void __launch_bounds__(kHnThreads) qk_norm_rope_bwd_kernel(const __grid_constant__ HeadNormArgs a) {
+  __shared__ float red[NORM ? kHnWarps : 1][2][kPdDim];
+  __shared__ __align__(16) float freq[ROPE ? 128 : 4];
+  const int lane = threadIdx.x & 31, c = lane & 7, hl = lane >> 3, warp = threadIdx.x >> 5;
+  if (ROPE) {
+    load_rot_table(a.rot, freq);
+    __syncthreads();
+  }
+  pdl_wait();
+  pdl_trigger();
+  float wq[16], wk[16], dwq[16], dwk[16];
+  load_weight<T, NORM>(a.wq, c, wq);
+  load_weight<T, NORM>(a.wk, c, wk);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) dwq[i] = dwk[i] = 0.f;
+  const long long units = static_cast<long long>(a.T) * a.splits;
+  for (long long unit = static_cast<long long>(blockIdx.x) * kHnWarps + warp; unit < units;
+       unit += static_cast<long long>(gridDim.x) * kHnWarps) {
+    const int t = static_cast<int>(unit / a.splits), sp = static_cast<int>(unit % a.splits);
+    float cs[8], sn[8];
+    token_rotation<ROPE>(a, freq, t, c, cs, sn);
+    const int first = sp * 4, step = 4 * a.splits;
+    const size_t oq = static_cast<size_t>(t) * a.Nq * kPdDim, ok = static_cast<size_t>(t) * a.Nk * kPdDim;
+    heads_backward<T, NORM, ROPE>(static_cast<const T*>(a.q) + t * a.q_stride, static_cast<const T*>(a.gq) + oq,
+                                  static_cast<T*>(a.yq) + oq, a.Nq, first, step, wq, dwq, cs, sn, c, hl, a.eps);
+    heads_backward<T, NORM, ROPE>(static_cast<const T*>(a.k) + t * a.k_stride, static_cast<const T*>(a.gk) + ok,
+                                  static_cast<T*>(a.yk) + ok, a.Nk, first, step, wk, dwk, cs, sn, c, hl, a.eps);
+  }
+  if (NORM) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int d = 8; d < 32; d <<= 1) {
+        dwq[i] += __shfl_xor_sync(0xffffffffu, dwq[i], d);
+        dwk[i] += __shfl_xor_sync(0xffffffffu, dwk[i], d);
+      }
+      if (hl == 0) {
+        const int dim = (i >> 3) * 64 + c * 8 + (i & 7);
+        red[warp][0][dim] = dwq[i];
+        red[warp][1][dim] = dwk[i];
+      }
+    }
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < kHnWarps; ++w) t += red[w][threadIdx.x >> 7][threadIdx.x & 127];
+    a.partial[static_cast<size_t>(blockIdx.x) * 2 * kPdDim + threadIdx.x] = t;
+  }
+}
+static_assert(kHnThreads == 2 * kPdDim, "a thread per element of the two weight gradients");
+
+// dwq and dwk: the parked rows added in a fixed order.  A CTA owns eight of the 256 columns; thread (r, col) adds the rows
+// r, r + 32, ... and the 32 sums of a column are added in a tree over the lanes that hold them.
+template <typename T>
+__global__ void __launch_bounds__(256) head_norm_dw_kernel(void* dwq, void* dwk, const float* __restrict__ partial, int rows) {
+  __shared__ float red[32][9];
+  const int col = threadIdx.x & 7, r = threadIdx.x >> 3;
+  pdl_wait();
+  pdl_trigger();
+  float t = 0.f;
+  for (int i = r; i < rows; i += 32) t += __ldcg(partial + static_cast<size_t>(i) * 2 * kPdDim + blockIdx.x * 8 + col);
+  red[r][col] = t;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float v = red[lane][warp];
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if (lane == 0) {
+    const int i = blockIdx.x * 8 + warp;
+    static_cast<T*>(i < kPdDim ? dwq : dwk)[i & (kPdDim - 1)] = static_cast<T>(v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// the served rows: normalised queries out, normalised keys and the values into the pages
+// ---------------------------------------------------------------------------------------------
+
+struct NormAppendArgs {
+  const void* q;            // [T, Nq, 128], rows q_stride elements apart
+  const void* k;            // [T, Nk, 128]
+  const void* v;
+  const void* wq;
+  const void* wk;
+  void* yq;                 // [T, Nq, 128] contiguous
+  const void* const* kv_ptrs;
+  const int32_t* kv_indptr;
+  const int32_t* last_page_offset;
+  const int32_t* append_indptr;   // [B + 1]; null: one token per request
+  int* err;
+  long long q_stride, k_stride, v_stride;
+  int T, batch, Nq, Nk, num_layers, layer_idx, page_size, total_pages, splits;
+  float eps;
+};
+
+// One warp per (token, share of its heads).
+template <typename T>
+__global__ void __launch_bounds__(kHnThreads) norm_append_kernel(const NormAppendArgs a) {
+  const int lane = threadIdx.x & 31, c = lane & 7, hl = lane >> 3;
+  pdl_wait();
+  pdl_trigger();
+  const long long unit = static_cast<long long>(blockIdx.x) * kHnWarps + (threadIdx.x >> 5);
+  const int t = static_cast<int>(unit / a.splits), sp = static_cast<int>(unit % a.splits);
+  if (t >= a.T) return;
+  // the request of the token: how many of them start at or before it (every lane looks at some, all loads at once)
+  int b = t, t0 = t, n = 1;
+  if (a.append_indptr != nullptr) {
+    int before = 0;
+    for (int i0 = 0; i0 < a.batch; i0 += 32) {
+      const int i = i0 + lane;
+      before += __popc(__ballot_sync(0xffffffffu, i < a.batch && a.append_indptr[i] <= t));
+    }
+    b = before - 1;
+    if (b < 0) return;                       // a row in front of the first request
+    t0 = a.append_indptr[b];
+    n = a.append_indptr[b + 1] - t0;
+    if (t - t0 >= n) return;                 // a row behind the last one
+  }
+  float wq[16], wk[16];
+  const float none[8] = {};
+  load_weight<T, true>(a.wq, c, wq);
+  load_weight<T, true>(a.wk, c, wk);
+  const int first = sp * 4, step = 4 * a.splits;
+  heads_forward<T, true, false, 2>(static_cast<const T*>(a.q) + t * a.q_stride,
+                                   static_cast<T*>(a.yq) + static_cast<size_t>(t) * a.Nq * kPdDim, a.Nq, first, step, wq,
+                                   none, none, c, hl, a.eps);
+  const int p0 = a.kv_indptr[b], p1 = a.kv_indptr[b + 1], P = a.page_size;
+  const int len = p1 > p0 ? (p1 - p0 - 1) * P + a.last_page_offset[b] : 0;
+  const int pos = len - n + (t - t0);
+  if (p0 < 0 || p1 > a.total_pages || pos < 0 || n > len || pos >= (p1 - p0) * P) {   // the pages do not hold the token
+    if (lane == 0 && a.err != nullptr) atomicOr(a.err, kErrBadIndptr);
+    return;
+  }
+  T* page = static_cast<T*>(const_cast<void*>(a.kv_ptrs[p0 + pos / P]));
+  if (page == nullptr || (reinterpret_cast<uintptr_t>(page) & 15) != 0) {
+    if (lane == 0 && a.err != nullptr) atomicOr(a.err, kErrBadPointer);
+    return;
+  }
+  // a head's place: [layer][key | value][head][entry][128]
+  const size_t head_step = static_cast<size_t>(P) * kPdDim;
+  T* kd = page + static_cast<size_t>(a.layer_idx) * 2 * a.Nk * head_step + static_cast<size_t>(pos % P) * kPdDim + c * 8;
+  const T* ks = static_cast<const T*>(a.k) + t * a.k_stride + c * 8;
+  const T* vs = static_cast<const T*>(a.v) + t * a.v_stride + c * 8;
+  for (int h0 = first; h0 < a.Nk; h0 += step) {
+    const int h = h0 + hl;
+    uint4 kl = make_uint4(0u, 0u, 0u, 0u), kh = kl, vl = kl, vh = kl;
+    if (h < a.Nk) {
+      kl = __ldg(reinterpret_cast<const uint4*>(ks + h * kPdDim));
+      kh = __ldg(reinterpret_cast<const uint4*>(ks + h * kPdDim + 64));
+      vl = __ldg(reinterpret_cast<const uint4*>(vs + h * kPdDim));
+      vh = __ldg(reinterpret_cast<const uint4*>(vs + h * kPdDim + 64));
+    }
+    float p[8], q[8];
+    unpack8<T>(kl, p);
+    unpack8<T>(kh, q);
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += p[i] * p[i] + q[i] * q[i];
+    const float s = rsqrtf(sum8(ss) * (1.0f / kPdDim) + a.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] *= s * wk[i];
+      q[i] *= s * wk[8 + i];
+    }
+    if (h < a.Nk) {
+      T* dst = kd + h * head_step;
+      *reinterpret_cast<uint4*>(dst) = pack8<T>(p);
+      *reinterpret_cast<uint4*>(dst + 64) = pack8<T>(q);
+      dst += a.Nk * head_step;
+      *reinterpret_cast<uint4*>(dst) = vl;
+      *reinterpret_cast<uint4*>(dst + 64) = vh;
+    }
+  }
+}
+
+}  // namespace smlm

@@ -1,0 +1,32 @@
+// The rotary embedding's angles at any position.
+#pragma once
+#include "smlm_common.cuh"
+
+namespace smlm {
+
+// The 64 frequencies in half-turns per position, base^(-2 i / 128) / pi, each as the sum of two floats: a product with
+// a position is then good to 2^-40 half-turns or so, where one float is off by several thousandths of a turn from
+// position 10^5 on - more than the rounding of a 16-bit result.
+struct RotTable {
+  float hi[64], lo[64];
+};
+
+// cos and sin of pi * pos * (hi + lo) for positions below 2^24 in absolute value
+__device__ __forceinline__ void rot_sincos(float pos, float hi, float lo, float* s, float* c) {
+  const float a = __fmul_rn(pos, hi);
+  const float e = __fmaf_rn(pos, lo, __fmaf_rn(pos, hi, -a));   // what a lacks
+  const float r = a - 2.0f * rintf(0.5f * a) + e;               // the difference of the first two is exact
+  *s = __sinf(3.14159265358979f * r);
+  *c = __cosf(3.14159265358979f * r);
+}
+
+
+// the table into shared memory, [hi | lo]; every thread of the CTA takes part, a barrier follows at the caller
+__device__ __forceinline__ void load_rot_table(const RotTable& rot, float* freq) {
+  for (int i = threadIdx.x; i < 64; i += blockDim.x) {
+    freq[i] = rot.hi[i];
+    freq[64 + i] = rot.lo[i];
+  }
+}
+
+}  // namespace smlm

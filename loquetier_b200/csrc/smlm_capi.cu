@@ -18,6 +18,7 @@
 #include "rms_norm.cuh"
 #include "smlm_fused.cuh"
 #include "smlm_fused_tc.cuh"
+#include "smlm_launch.cuh"
 #include "smlm_merge.cuh"
 #include "smlm_plan.cuh"
 #include "smlm_wgrad.cuh"
@@ -26,8 +27,6 @@
 namespace {
 
 using namespace smlm;
-
-constexpr int kNumSMs = 148;
 
 
 // ---- tensor maps ------------------------------------------------------------
@@ -104,8 +103,6 @@ bool make_map_2d(CUtensorMap* m, const void* base, int rows, int cols, int box_r
   return true;
 }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 // Rows per piece for a batch of T rows.  The plan builder and every launch derive it from T alone,
 // so they always agree.  64 everywhere: cutting 8192 rows into 56-row pieces would give each of the
 // 148 SMs one piece of a uniform batch, but with ragged segments the remainders spill into a second
@@ -126,68 +123,6 @@ inline int tall_rows_for(int T, int nseg) {
   return 2 * kBM;
 }
 inline int max_tall_pieces_of(int T, int nseg) { return T / tall_rows_for(T, nseg) + nseg; }
-
-// The opt-in to more than 48 KB of dynamic shared memory is a property of (kernel, device): it is
-// set when a kernel is first launched on a device, or with more shared memory than before, and
-// remembered - not repeated per launch.
-constexpr int kMaxDevices = 64;
-std::mutex g_attr_mutex;
-std::vector<std::pair<const void*, int>> g_attr_done[kMaxDevices];
-
-bool ensure_dynamic_smem(const void* kern, int smem_bytes) {
-  int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
-    cudaGetLastError();
-    return false;
-  }
-  {
-    std::lock_guard<std::mutex> lock(g_attr_mutex);
-    for (const auto& k : g_attr_done[dev])
-      if (k.first == kern && k.second >= smem_bytes) return true;
-  }
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  std::lock_guard<std::mutex> lock(g_attr_mutex);
-  for (auto& k : g_attr_done[dev])
-    if (k.first == kern) {
-      k.second = std::max(k.second, smem_bytes);
-      return true;
-    }
-  g_attr_done[dev].emplace_back(kern, smem_bytes);
-  return true;
-}
-
-template <typename Kern, typename... Args>
-int launch(Kern kern, dim3 grid, int threads, int cluster_x, int smem_bytes, cudaStream_t stream,
-           const Args&... args) {
-  if (grid.x == 0 || grid.y == 0) return SMLM_OK;
-  // the limit without the opt-in is 48 KB for dynamic and static shared memory TOGETHER, hence the margin
-  if (smem_bytes > 40 * 1024 && !ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem_bytes))
-    return SMLM_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster_x;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  // every kernel of the library calls pdl_wait() before it touches memory that an earlier kernel
-  // of the stream may have written, so it may be scheduled while its predecessor drains
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
-    cudaGetLastError();
-    return SMLM_ERR_CUDA;
-  }
-  return SMLM_OK;
-}
 
 // ---- fused shrink + expand ----------------------------------------------------
 
@@ -742,10 +677,6 @@ int dispatch_prefill(const PfArgs& a, const CUtensorMap& kvmap, int group, cudaS
     case 8: return launch(paged_prefill_kernel<T, 8>, grid, kPfThreads, 1, kPfSmem, stream, a, kvmap);
     default: return SMLM_ERR_NO_KERNEL;
   }
-}
-
-inline bool kv_shape_ok(int head_dim, int page_size) {
-  return head_dim == kPdDim && (page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64);
 }
 
 int run_append(const void* const* kv_ptrs, const int32_t* kv_indptr, const int32_t* last_page_offset, const void* k,

@@ -16,7 +16,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
-from torch.autograd.function import Function, FunctionCtx
+from torch.autograd.function import Function, FunctionCtx, once_differentiable
 
 from . import ops
 
@@ -158,6 +158,66 @@ class rms_norm(Function):
             return dx, dw.zero_(), None
         ops.rms_norm_bwd(dx, dw, go, x, w, rms_1)
         return dx, dw, None
+
+
+class qk_norm_rope(Function):
+    """``qk_norm_rope.apply(q, k, q_weight, k_weight, positions, base, eps)`` -> (q', k'): per token and head the RMSNorm over
+    head_dim (both weights given, else both None) and the rotary embedding at ``positions`` (int32 or int64 per token, below
+    2^24; None: not rotated), in one pass over each direction.  For rows that are trained; rows on their way into the
+    cache take ``kvcache.norm_append_kv``.
+
+    ``q`` ``[tokens, num_heads, 128]`` and ``k`` ``[tokens, num_kv_heads, 128]``, fp16 or bf16, may be slices of one projection;
+    results and their gradients are contiguous.  Weight gradients are summed in fp32 in a fixed order."""
+
+    @staticmethod
+    def forward(ctx: FunctionCtx, q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
+                k_weight: Optional[torch.Tensor], positions: Optional[torch.Tensor], base: float = 10000.0,
+                eps: float = 1e-6):
+        for t, name in ((q, "q"), (k, "k")):
+            ops.row_stride(t, name, ops.HEAD_DIM)
+        if k.size(0) != q.size(0) or q.size(1) == 0 or k.size(1) == 0:
+            raise RuntimeError("q and k must have the same number of rows, and heads")
+        if (q_weight is None) != (k_weight is None):
+            raise RuntimeError("q_weight and k_weight must be given together")
+        if q_weight is None and positions is None:
+            raise RuntimeError("neither weights nor positions are given: nothing to do")
+        for t, name in ((k, "k"), (q_weight, "q_weight"), (k_weight, "k_weight")):
+            if t is not None and t.dtype != q.dtype:
+                raise RuntimeError(f"{name} must be {q.dtype} like q")
+        for t, name, n in ((q_weight, "q_weight", ops.HEAD_DIM), (k_weight, "k_weight", ops.HEAD_DIM),
+                           (positions, "positions", q.size(0))):
+            if t is not None:
+                ops._chk_cuda_contig(t, name, 1)
+                if t.numel() != n:
+                    raise RuntimeError(f"{name} must hold {n} values")
+        if positions is not None and positions.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError("positions must be int32 or int64")
+        for t in (k, q_weight, k_weight, positions):
+            if t is not None and t.device != q.device:
+                raise RuntimeError(f"every tensor must be on {q.device}")
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions)
+        ctx.base, ctx.eps = base, eps
+        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        return ops.qk_norm_rope(yq, yk, q, k, q_weight, k_weight, positions, base, eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: FunctionCtx, grad_q: torch.Tensor, grad_k: torch.Tensor):
+        q, k, wq, wk, positions = ctx.saved_tensors
+        # autograd's own nodes behind this one cannot be captured while an eager graph of the same leaves lives
+        ops.refuse_capture(q, "the backward of qk_norm_rope")
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dwq, dwk = (None, None) if wq is None else (torch.empty_like(wq), torch.empty_like(wk))
+        if q.size(0) == 0:
+            if wq is not None:
+                dwq.zero_()
+                dwk.zero_()
+        else:
+            ops.qk_norm_rope_bwd(dq, dk, dwq, dwk, grad_q.contiguous(), grad_k.contiguous(), q, k, wq, wk, positions,
+                                 ctx.base, ctx.eps)
+        return dq, dk, dwq, dwk, None, None, None
 
 
 class MixedLlamaRMSNorm(torch.nn.Module):

@@ -88,6 +88,18 @@ def _chk_cuda_contig(t: torch.Tensor, name: str, dim: int):
         raise RuntimeError(f"{name} must be a {dim}D tensor")
 
 
+def row_stride(t: torch.Tensor, name: str, head_dim: int) -> int:
+    """Elements from one row of ``t`` ``[rows, heads, head_dim]`` to the next, for operators that take slices of a wider
+    projection: the heads of a row must be contiguous."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dim() != 3 or t.size(2) != head_dim:
+        raise RuntimeError(f"{name} must be [rows, heads, {head_dim}]")
+    if t.stride(2) != 1 or (t.size(1) > 1 and t.stride(1) != head_dim):
+        raise RuntimeError(f"the heads of a row of {name} must be contiguous")
+    return int(t.stride(0)) if t.size(0) > 1 else int(t.size(1)) * head_dim
+
+
 class Plan:
     """Work list of one batch: built on the device from the segment index pointer,
     shared by every SMLM call of the batch (all projections, shrink and expand)."""
@@ -413,3 +425,37 @@ def rms_norm_bwd(dx: torch.Tensor, dw: torch.Tensor, go: torch.Tensor, x: torch.
                                          rms.data_ptr(), ws.data_ptr(), ws.numel(), rows, cols, _dtype_code(x),
                                          int(dw.dtype == torch.float32), _stream(x)), "smlm_b200_rms_norm_bwd")
     return dx, dw
+
+
+# ---------------------------------------------------------------------------
+# norms of queries and keys per head, with the rotary embedding
+# ---------------------------------------------------------------------------
+
+HEAD_DIM = 128
+
+
+def qk_norm_rope(yq, yk, q, k, wq, wk, positions, base: float, eps: float):
+    """yq, yk = q, k normalised per head (weights given) and rotated (positions given); q and k may be strided rows."""
+    with on_device(q):
+        check(lib.smlm_b200_qk_norm_rope(yq.data_ptr(), yk.data_ptr(), q.data_ptr(), k.data_ptr(), _p(wq), _p(wk),
+                                         _p(positions), row_stride(q, "q", HEAD_DIM), row_stride(k, "k", HEAD_DIM),
+                                         int(q.size(0)), int(q.size(1)), int(k.size(1)), HEAD_DIM,
+                                         int(positions is not None and positions.dtype == torch.int64), float(base),
+                                         float(eps), _dtype_code(q), _stream(q)), "smlm_b200_qk_norm_rope")
+    return yq, yk
+
+
+def qk_norm_rope_bwd(dq, dk, dwq, dwk, gq, gk, q, k, wq, wk, positions, base: float, eps: float,
+                     workspace: Optional[torch.Tensor] = None):
+    """Gradients of ``qk_norm_rope``; gq, gk, dq and dk contiguous, dwq and dwk in the storage type (None without weights)."""
+    T, Nq, Nk = int(q.size(0)), int(q.size(1)), int(k.size(1))
+    if workspace is None and wq is not None:
+        workspace = torch.empty(int(lib.smlm_b200_qk_norm_rope_bwd_workspace_bytes(T, Nq, Nk)), dtype=torch.uint8,
+                                device=q.device)
+    with on_device(q):
+        check(lib.smlm_b200_qk_norm_rope_bwd(dq.data_ptr(), dk.data_ptr(), _p(dwq), _p(dwk), gq.data_ptr(), gk.data_ptr(),
+                                             q.data_ptr(), k.data_ptr(), _p(wq), _p(wk), _p(positions), _p(workspace),
+                                             0 if workspace is None else workspace.numel(), row_stride(q, "q", HEAD_DIM),
+                                             row_stride(k, "k", HEAD_DIM), T, Nq, Nk, HEAD_DIM,
+                                             int(positions is not None and positions.dtype == torch.int64), float(base),
+                                             float(eps), _dtype_code(q), _stream(q)), "smlm_b200_qk_norm_rope_bwd")
