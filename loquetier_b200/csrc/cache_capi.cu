@@ -29,46 +29,41 @@ const RotTable& rot_table(double base) {
   return table;
 }
 
-// How an extend launch is laid out: everything follows from sizes the host knows, so that the workspace query and the launch agree.
+// How an extend launch is laid out: everything follows from sizes the host knows, so that the workspace query and the launch
+// agree.
 struct ExPlan {
-  int nt;          // column tiles of eight rows per row tile
-  int rows;        // rows of a tile
-  int target;      // ranges aimed at per kv head
-  int min_tiles;   // key tiles of a range at least
-  int slots;       // (tile, range) pairs per kv head
-  bool merge;      // a tile may have several ranges
-  size_t bytes;    // of parked states
+  int qt;          // quarters of 32 rows of a row tile
+  int shares;      // CTAs per kv head
+  int min_tiles;   // key tiles of a share at least
+  size_t bytes;    // of softmax states
 };
 
 ExPlan extend_plan(int batch, int total_q, int total_pages, int page_size, int num_kv_heads, int group) {
   ExPlan p;
   const long long all_rows = static_cast<long long>(total_q) * group;
   const long long mean = (all_rows + batch - 1) / batch;
-  p.nt = mean <= 8 ? 1 : mean <= 16 ? 2 : 4;
-  p.rows = ex_rows(p.nt);
-  p.min_tiles = kPdWarps;
-  const long long key_tiles = static_cast<long long>(total_pages) * page_size / kPdTile + 1;
-  const long long tiles = all_rows / p.rows + batch;
-  const long long most = (all_rows / p.rows + 1) * key_tiles / p.min_tiles + 1;
-  const long long want = std::max(1, 2 * kNumSMs * ex_ctas_per_sm(p.nt) / num_kv_heads);
-  p.target = static_cast<int>(std::min(want, most));
-  p.slots = static_cast<int>(std::min<long long>(tiles + p.target, 0x7fffffffLL / num_kv_heads));
-  p.merge = key_tiles > p.min_tiles;
-  p.bytes = p.merge ? static_cast<size_t>(p.slots) * num_kv_heads * p.rows * kPdRec * sizeof(float) : 0;
+  p.qt = mean <= 32 ? 1 : mean <= 64 ? 2 : 4;
+  p.min_tiles = 4;
+  const int rows = 32 * p.qt;
+  // all the CTAs that are resident, but no more than the work can hold
+  const long long key_tiles = static_cast<long long>(total_pages) * page_size / kXtKeys + batch;
+  const long long most = (all_rows / rows + batch) * key_tiles / p.min_tiles + 1;
+  p.shares = static_cast<int>(std::min<long long>(std::max(1, kXtCtasPerSm * kNumSMs / num_kv_heads), most));
+  p.bytes = p.shares > 1 ? static_cast<size_t>(p.shares) * num_kv_heads * (sizeof(ExCut) + 2 * rows * kPdRec * sizeof(float)) : 0;
   return p;
 }
 
-template <typename T, int NT>
+template <typename T, int QT>
 int launch_extend(const ExArgs& a, const ExPlan& p, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.slots) * a.num_kv_heads, 1, 1);
-  const int rc = launch(paged_extend_kernel<T, NT>, grid, kExThreads, 1, ex_smem(NT), stream, a);
-  if (rc != SMLM_OK || !p.merge) return rc;
-  return launch(paged_extend_merge_kernel<T, 8 * NT, kPdTile>, grid, kExThreads, 1, 0, stream, a);
+  const unsigned heads = static_cast<unsigned>(a.num_kv_heads);
+  const int rc = launch(paged_extend_kernel<T, QT>, dim3(p.shares * heads, 1, 1), Xt<QT>::kThreads, 1, Xt<QT>::kSmem, stream, a);
+  if (rc != SMLM_OK || p.shares == 1) return rc;
+  return launch(paged_extend_merge_kernel<T, QT>, dim3((p.shares - 1) * heads, kXtMergeSplit, 1), kXtMergeThreads, 1, 0, stream, a);
 }
 
 template <typename T>
 int dispatch_extend(const ExArgs& a, const ExPlan& p, cudaStream_t stream) {
-  switch (p.nt) {
+  switch (p.qt) {
     case 1: return launch_extend<T, 1>(a, p, stream);
     case 2: return launch_extend<T, 2>(a, p, stream);
     default: return launch_extend<T, 4>(a, p, stream);
@@ -155,7 +150,8 @@ int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, con
     return SMLM_ERR_INVALID_ARGUMENT;
   if (!aligned16(o) || !aligned16(q)) return SMLM_ERR_MISALIGNED;
   if (static_cast<long long>(total_q) * num_qo_heads > 0x7fffffffLL ||
-      static_cast<long long>(total_pages) * page_size > 0x7fffffffLL)
+      static_cast<long long>(total_pages) * page_size > 0x7fffffffLL ||
+      static_cast<long long>(num_layers) * 2 * num_kv_heads * page_size * kPdDim * 2 > 0x7fffffffLL)   // a page of 2 GB
     return SMLM_ERR_INVALID_ARGUMENT;
   const ExPlan p = extend_plan(batch_size, total_q, total_pages, page_size, num_kv_heads, group);
   if (p.bytes > 0) {
@@ -164,11 +160,13 @@ int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, con
   }
   ExArgs a;
   a.o = o; a.q = q; a.qo_indptr = qo_indptr; a.kv_ptrs = kv_ptrs; a.kv_indptr = kv_indptr;
-  a.last_page_offset = last_page_offset; a.partial = static_cast<float*>(workspace); a.err = status_word;
+  a.last_page_offset = last_page_offset; a.err = status_word;
+  a.cuts = p.bytes > 0 ? static_cast<ExCut*>(workspace) : nullptr;
+  a.partial = reinterpret_cast<float*>(a.cuts + static_cast<size_t>(p.shares) * num_kv_heads);
   a.batch = batch_size; a.total_q = total_q; a.total_pages = total_pages; a.num_kv_heads = num_kv_heads;
   a.num_layers = num_layers; a.layer_idx = layer_idx; a.page_size = page_size;
   a.lg = group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3;
-  a.target = p.target; a.min_tiles = p.min_tiles; a.slots = p.slots;
+  a.shares = p.shares; a.min_tiles = p.min_tiles;
   a.rot = rot_table(rope_theta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == SMLM_F16 ? dispatch_extend<__half>(a, p, st) : dispatch_extend<__nv_bfloat16>(a, p, st);

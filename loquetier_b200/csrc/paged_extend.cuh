@@ -3,19 +3,45 @@
 //
 //   o[i, h] = sum_{j <= p_i} softmax_j( R(p_i) q[i, h] . R(j) k_j / sqrt(128) ) v_j,     p_i = L - n + i
 //
-// for the n new tokens of a request of L keys, which the cache already holds, un-rotated.  The pages are read in place.
-// The rows of a request and kv head are its n * G (query, head) pairs, row = query * G + head of the group; they are cut into
-// tiles, and the keys of a tile into ranges where there are too few tiles to fill the machine (few new tokens on a
-// long cache).  A CTA owns one (tile, kv head, range).  Which one it finds for itself: the lengths live on the device.  The
-// ranges follow from the lengths alone, so the same batch gives the same result; parked softmax states of a tile
-// with several ranges are merged by a second launch, in range order.
+// for the n new tokens of a request of L keys, which the cache already holds, un-rotated.
+//
+// The rows of a request and kv head are its n * G (query, head) pairs, row = query * G + head of the group, cut into tiles
+// of 32 QT rows; the keys are cut into tiles of 64.  All (request, row tile, key tile) triples of a kv head, in this order,
+// are the work, and every CTA of that head takes an even, contiguous share of it: a long cache is spread over many CTAs,
+// several short ones follow one another in one, and the launch is one wave that ends everywhere at once whatever the
+// lengths.  A CTA finds its share itself, because the lengths live on the device.  A row tile that lies in one share is finished
+// there; one that is cut leaves a softmax state per share, merged by a second launch in the order of the keys.  The cuts
+// follow from the lengths alone: the same batch gives the same result.
+//
+//   S[128, 64]   = Q . K_tile^T    tcgen05.mma, both operands K-major in shared memory, two accumulators in tensor memory
+//   P            = exp2(S - m)     a row is a tensor-memory lane, two threads per row
+//   O[128, 128] += P . V_tile      A = P in tensor memory, B = V MN-major as the cache stores it
+//
+// The products and the softmax are those of the prefill kernel (paged_prefill.cuh).  What differs is where the tiles come
+// from: here loader warps fetch K and V from the pages themselves with 16-byte asynchronous copies, straight into the
+// swizzled places the products read, and rotate the keys in place.  A loader thread has eight frequencies (dimensions
+// 8 c .. 8 c + 7 and their partners) and a fixed distance between its keys, so its cosines and sines go on from key to key
+// by one turn.  It waits for its own copies only, and runs ahead across row tiles and requests.
+//
+// The products always have 128 rows; what lies behind the tile's rows in shared memory feeds accumulator lanes that nobody
+// reads.  Softmax warps are those whose tensor-memory lanes hold the tile's rows, the loaders and the two issuers the others.
+// Every wait is bounded.
 #pragma once
-#include "paged_kv.cuh"
+#include "paged_prefill.cuh"
 #include "rotary.cuh"
 
 namespace smlm {
 
-constexpr int kExThreads = 128;
+constexpr int kXtKeys = 64;
+constexpr int kXtCtasPerSm = 2;
+constexpr int kXtTileBytes = kXtKeys * kPdDim * 2;      // two 64-dim panels of [64 keys][128 B]
+constexpr int kXtPanel = kXtKeys * 128;
+constexpr int kXtOCol = 2 * kXtKeys;                    // tensor memory: two S buffers, then O
+constexpr int kXtTmemCols = 256;
+constexpr int kXtHalf = kXtKeys / 2;                    // columns of S per softmax thread
+constexpr int kXtReseed = 16;                           // tiles after which the rotation is computed afresh
+
+struct ExCut;
 
 struct ExArgs {
   void* o;                        // [total_q, Nq, 128]
@@ -24,32 +50,27 @@ struct ExArgs {
   const void* const* kv_ptrs;
   const int32_t* kv_indptr;       // [B + 1]
   const int32_t* last_page_offset;  // [B]
-  float* partial;                 // [slots * Nkv][rows of a tile][kPdRec]
+  float* partial;                 // states [shares][2][Nkv][rows of a tile][kPdRec]: a share cuts two row tiles at most
+  ExCut* cuts;                    // [shares][Nkv]
   int* err;                       // error word, may be null
   int batch, total_q, total_pages, num_kv_heads, num_layers, layer_idx, page_size;
   int lg;                         // log2 of the query heads per kv head, G
-  int target;                     // ranges aimed at per kv head
-  int min_tiles;                  // a range has this many key tiles at least
-  int slots;                      // (tile, range) pairs per kv head that the launch and the workspace provide for
+  int shares;                     // CTAs per kv head
+  int min_tiles;                  // a share has this many key tiles at least
   RotTable rot;
 };
 
-struct ExItem {
-  int b;          // request; negative: the slot is not used
-  int tile;       // of its rows
-  int range, ranges;
-  int slot0;      // the slot of the tile's first range
+struct ExRequest {
   int qo0, n;     // first row of q, new tokens
   int p0, len;    // first page in the table, keys
-  int per;        // key tiles of a range
   int bad;        // error bits of its entries in the index arrays
 };
 
-// a request's rows and keys, with the index arrays checked
-__device__ __forceinline__ void ex_request(const ExArgs& a, int b, ExItem& r) {
+__device__ __forceinline__ ExRequest ex_request(const ExArgs& a, int b) {
   const int q0 = a.qo_indptr[b], q1 = a.qo_indptr[b + 1];
   const int p0 = a.kv_indptr[b], p1 = a.kv_indptr[b + 1];
   const int last = a.last_page_offset[b];
+  ExRequest r;
   r.bad = 0;
   r.qo0 = q0;
   r.n = q1 - q0;
@@ -64,486 +85,731 @@ __device__ __forceinline__ void ex_request(const ExArgs& a, int b, ExItem& r) {
     r.bad = kErrBadIndptr;
   }
   if (r.len < r.n) r.bad = kErrBadIndptr;   // more queries than keys
+  return r;
 }
+template <int ROWS>
+__device__ __forceinline__ int ex_row_tiles(const ExArgs& a, const ExRequest& r) {
+  return ((r.n << a.lg) + ROWS - 1) / ROWS;
+}
+// key tiles of each of a request's row tiles (one at least: rows that see no key still have to be written)
+__device__ __forceinline__ int ex_key_tiles(const ExRequest& r) { return max(1, (r.len + kXtKeys - 1) / kXtKeys); }
 
-// The (tile, range) that slot `slot` stands for.  ROWS rows and KEYS keys are a tile.  Requests come in order, a request's
-// tiles in order, a tile's ranges in order.  Two passes over the requests: the batch's work gives the length of a range, the
-// numbers of ranges the places.  Every thread of the CTA takes part; `report`: one of them writes down what is wrong with the
-// index arrays.
-template <int ROWS, int KEYS, int NT>
-__device__ __forceinline__ ExItem ex_find(const ExArgs& a, int slot, bool report) {
-  __shared__ long long s_sum[NT / 32];
-  __shared__ int s_scan[NT / 32];
-  __shared__ ExItem s_item;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  ExItem r;
-  long long work = 0;
-  for (int b = tid; b < a.batch; b += NT) {
-    ex_request(a, b, r);
-    if (report && r.bad != 0 && a.err != nullptr) atomicOr(a.err, r.bad);
-    if (r.n > 0) work += static_cast<long long>(((r.n << a.lg) + ROWS - 1) / ROWS) * ((r.len + KEYS - 1) / KEYS);
-  }
+// A run of key tiles of one row tile.
+struct ExSeg {
+  int qo0, row0, nrows;   // first row of q of the request; of its rows, the tile's first and their number
+  int pos0, p0;           // position of the request's first new token; first page in the table
+  int nkeys;              // keys that a row of the tile sees
+  int tile0, ntiles;      // the run, cut where no row sees a key any more (one tile at least of a row tile's first run)
+  int part;               // where its state goes: 0, 1, or negative: the row tile is finished here
+};
+
+template <int SEGS>
+struct ExScratch {
+  long long sum[16];
+  long long begin, end, next;   // of the share's work; where the next round of runs starts
+  int count;
+  ExSeg seg[SEGS];              // runs of the share that are laid out at a time
+};
+
+// the sum over the CTA's NT threads
+template <int NT, typename S>
+__device__ __forceinline__ long long ex_sum(long long v, S& sc) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) work += __shfl_xor_sync(0xffffffffu, work, d);
-  if (lane == 0) s_sum[warp] = work;
-  if (tid == 0) s_item.b = -1;
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   __syncthreads();
-  work = 0;
+  if ((threadIdx.x & 31) == 0) sc.sum[threadIdx.x >> 5] = v;
+  __syncthreads();
+  long long t = 0;
 #pragma unroll
-  for (int w = 0; w < NT / 32; ++w) work += s_sum[w];
-  const long long even = (work + a.target - 1) / a.target;
-  const int per = static_cast<int>(even > a.min_tiles ? even : a.min_tiles);
-  int before = 0;
-  for (int b0 = 0; b0 < a.batch && before <= slot; b0 += NT) {
-    const int b = b0 + tid;
-    int tiles = 0, ranges = 0;
-    if (b < a.batch) {
-      if (a.batch > NT) ex_request(a, b, r);   // (else r still holds it)
-      tiles = ((r.n << a.lg) + ROWS - 1) / ROWS;
-      ranges = max(1, ((r.len + KEYS - 1) / KEYS + per - 1) / per);
-    }
-    const int mine = tiles * ranges;
-    int incl = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += up;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    int base = before, all = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-      if (w < warp) base += s_scan[w];
-      all += s_scan[w];
-    }
-    const int excl = base + incl - mine;
-    if (mine > 0 && slot >= excl && slot - excl < mine) {
-      const int local = slot - excl;
-      r.b = b;
-      r.tile = local / ranges;
-      r.range = local % ranges;
-      r.ranges = ranges;
-      r.slot0 = slot - r.range;
-      r.per = per;
-      s_item = r;
-    }
-    before += all;
-    __syncthreads();
-  }
-  return s_item;
+  for (int w = 0; w < NT / 32; ++w) t += sc.sum[w];
+  return t;
 }
 
-// ---------------------------------------------------------------------------------------------
-// few rows: mma.sync with the keys as the rows of the tile
-// ---------------------------------------------------------------------------------------------
+// Key tiles of a share.  Every thread of the CTA takes part; `report`: what is wrong with the index arrays is written down.
+template <int ROWS, int NT, typename S>
+__device__ __forceinline__ long long ex_share(const ExArgs& a, bool report, S& sc) {
+  long long work = 0;
+  for (int b = threadIdx.x; b < a.batch; b += NT) {
+    const ExRequest r = ex_request(a, b);
+    if (report && r.bad != 0 && a.err != nullptr) atomicOr(a.err, r.bad);
+    work += static_cast<long long>(ex_row_tiles<ROWS>(a, r)) * ex_key_tiles(r);
+  }
+  work = ex_sum<NT>(work, sc);
+  const long long even = (work + a.shares - 1) / a.shares;
+  return even > a.min_tiles ? even : a.min_tiles;
+}
 
-constexpr int kExRing = kPdWarps * kPdWarpRing;
-constexpr int ex_rows(int nt) { return 8 * nt; }       // rows of a tile
-// ring, queries, turns by 64 and by 8 keys, frequencies
-constexpr int ex_smem(int nt) { return kExRing + ex_rows(nt) * kPdDim * 2 + 2 * 512 + 512; }
-constexpr int ex_ctas_per_sm(int nt) { return nt >= 4 ? 2 : 3; }
+// Running sums over the CTA's threads in their order: returns what the threads before this one hold, `all` the whole.
+template <int NT, typename S>
+__device__ __forceinline__ long long ex_scan(long long v, long long& all, S& sc) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long incl = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += up;
+  }
+  __syncthreads();
+  if (lane == 31) sc.sum[warp] = incl;
+  __syncthreads();
+  long long base = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) {
+    if (w < warp) base += sc.sum[w];
+    all += sc.sum[w];
+  }
+  return base + incl - v;
+}
 
-// Like the decode kernel, with 8 NT rows in place of the heads of one token:
-//   S^T[16 keys, 8 NT rows] = K . Q^T      O^T[128, 8 NT rows] += V^T . P^T       mma.sync m16n8k16
-// Each warp streams every fourth tile of 16 keys through a ring of its own; a key is rotated once, in registers, for all
-// rows.  Rotated keys and queries and the weights are rounded to 16 bits, the operands of the products; scores, maxima and
-// sums are fp32.
-template <typename T, int NT>
-__global__ void __launch_bounds__(kExThreads, ex_ctas_per_sm(NT)) paged_extend_kernel(const __grid_constant__ ExArgs a) {
-  extern __shared__ __align__(128) unsigned char ex_smem_buf[];
-  constexpr int ROWS = 8 * NT;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, t = lane & 3;       // MMA fragment coordinates: row g, column pair t
-  const uint32_t sbase = smem_u32(ex_smem_buf);
-  const uint32_t qs = sbase + kExRing;
-  float* rot = reinterpret_cast<float*>(ex_smem_buf + kExRing + ROWS * kPdDim * 2);
-  float* freq = rot + 256;
-  load_rot_table(a.rot, freq);
+// What the merge of the row tile that a share starts inside of needs to know.
+struct ExCut {
+  int qo0, row0, nrows;   // as in ExSeg; no rows: the share starts a row tile, or holds no work
+  int first, count;       // the row tile's first share, and the number of its shares whose rows see a key
+  int shares;             // all of its shares but the first: that many CTAs merge
+  int part;               // where the first share has its state; the others have it at 0
+  int pad;
+};
+
+// keys that a row of row tile `tile` of the request sees
+template <int ROWS>
+__device__ __forceinline__ int ex_visible(const ExArgs& a, const ExRequest& r, int tile) {
+  const int last = min((r.n << a.lg), (tile + 1) * ROWS) - 1;
+  return max(0, min(r.len, r.len - r.n + (last >> a.lg) + 1));
+}
+
+// Lays out the share's runs from `w0` on, in order, as many as fit.  The first round also writes down the cut that the
+// share starts with (cut: its place, null for other rounds).
+template <int ROWS, int NT, int SEGS>
+__device__ __forceinline__ void ex_layout(const ExArgs& a, long long w0, long long per, ExCut* cut, ExScratch<SEGS>& sc) {
+  const long long w_begin = sc.begin, w_end = sc.end;
+  if (threadIdx.x == 0) sc.next = w_end;
+  long long before = 0, segs = 0;
+  bool wrote = false;
+  for (int b0 = 0; b0 < a.batch && before < w_end && segs < SEGS; b0 += NT) {
+    const int b = b0 + threadIdx.x;
+    ExRequest r = {};
+    long long mine = 0;
+    int nt = 1;
+    if (b < a.batch) {
+      r = ex_request(a, b);
+      nt = ex_key_tiles(r);
+      mine = static_cast<long long>(ex_row_tiles<ROWS>(a, r)) * nt;
+    }
+    long long all, all_segs;
+    const long long at = before + ex_scan<NT>(mine, all, sc);
+    const long long from = max(w0, at), to = min(w_end, at + mine);
+    const int first = from < to ? static_cast<int>((from - at) / nt) : 0;          // row tiles in the share
+    const int n = from < to ? static_cast<int>((to - 1 - at) / nt) - first + 1 : 0;
+    long long i = segs + ex_scan<NT>(n, all_segs, sc);
+    for (int tile = first; tile < first + n && i < SEGS; ++tile, ++i) {
+      const long long start = at + static_cast<long long>(tile) * nt;
+      const int k0 = static_cast<int>(max(from, start) - start), k1 = static_cast<int>(min(to, start + nt) - start);
+      ExSeg s;
+      s.qo0 = r.qo0;
+      s.row0 = tile * ROWS;
+      s.nrows = min(ROWS, (r.n << a.lg) - s.row0);
+      s.pos0 = r.len - r.n;
+      s.p0 = r.p0;
+      s.nkeys = ex_visible<ROWS>(a, r, tile);
+      const int seen = max(1, (s.nkeys + kXtKeys - 1) / kXtKeys);
+      s.tile0 = k0;
+      s.ntiles = max(0, min(k1, seen) - k0);
+      s.part = k0 == 0 && k1 == nt ? -1 : start + k0 == w_begin ? 0 : 1;
+      sc.seg[i] = s;
+      if (i == SEGS - 1) sc.next = start + k1;
+      if (cut != nullptr && i == 0 && k0 > 0) {
+        ExCut c;
+        c.qo0 = s.qo0; c.row0 = s.row0; c.nrows = s.nrows;
+        c.first = static_cast<int>(start / per);
+        c.shares = static_cast<int>((start + nt - 1) / per) - c.first;
+        c.count = static_cast<int>((start + seen - 1) / per) - c.first + 1;
+        c.part = start == c.first * per ? 0 : 1;
+        c.pad = 0;
+        *cut = c;
+        wrote = true;
+      }
+    }
+    segs += all_segs;
+    before += all;
+  }
+  if (cut != nullptr && !__syncthreads_or(wrote) && threadIdx.x == 0) cut->nrows = 0;
+  __syncthreads();
+  if (threadIdx.x == 0) sc.count = static_cast<int>(min(segs, static_cast<long long>(SEGS)));
+  __syncthreads();
+}
+
+template <int QT>
+struct Xt {
+  static constexpr int kRows = 32 * QT;
+  static constexpr int kStages = QT == 4 ? 2 : 3;       // of the K ring and of the V ring
+  static constexpr int kSegs = QT == 2 ? 4 : 16;
+  static constexpr int kRotWarps = 4;
+  static constexpr int kThreads = 32 * (2 * QT + kRotWarps + 4);
+  static constexpr int kQPanel = kRows * 128;           // Q: two 64-dim panels of [rows][128 B]
+  static constexpr int kKOff = 2 * kQPanel;
+  static constexpr int kVOff = kKOff + kStages * kXtTileBytes;
+  static constexpr int kBarOff = kVOff + kStages * kXtTileBytes;
+  static constexpr int kBars = 5 * kStages + 7;
+  static constexpr int kTurnOff = (kBarOff + kBars * 8 + 8 + 15) / 16 * 16;
+  static constexpr int kScratchOff = kTurnOff + 512;
+  static constexpr int kSmem = kScratchOff + static_cast<int>(sizeof(ExScratch<kSegs>));
+  static_assert(kXtCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory budget");
+  static_assert(kQPanel + 128 * 128 <= kBarOff, "the products read 128 rows of each panel of Q");
+};
+
+// Eight keys of a tile, E the group's number: a lane copies 16 bytes of each second one, 512 bytes apart in the page, to the
+// four places of the group in `dst` (the same in every group but for 1024 bytes)
+template <int E>
+__device__ __forceinline__ void copy_eight(const uint32_t (&dst)[4], uint32_t off, uint64_t src) {
+  asm volatile("cp.async.cg.shared.global [%0 + %5], [%4], 16;\n"
+               "cp.async.cg.shared.global [%1 + %5], [%4 + 512], 16;\n"
+               "cp.async.cg.shared.global [%2 + %5], [%4 + 1024], 16;\n"
+               "cp.async.cg.shared.global [%3 + %5], [%4 + 1536], 16;\n"
+               ::"r"(dst[0] + off), "r"(dst[1] + off), "r"(dst[2] + off), "r"(dst[3] + off), "l"(src), "n"(E * 1024) : "memory");
+}
+__device__ __forceinline__ void lds128(uint32_t at, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// an entry of the page table, zero where there is none to read; without a branch, so that nothing waits for it here
+__device__ __forceinline__ uint64_t load_if(const void* const* at, bool yes) {
+  uint64_t v;
+  asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %2, 0;\nmov.b64 %0, 0;\n@p ld.global.nc.b64 %0, [%1];\n}\n"
+               : "=l"(v) : "l"(at), "r"(static_cast<int>(yes)));
+  return v;
+}
+
+// grid: shares * Nkv
+template <typename T, int QT>
+__global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_kernel(const __grid_constant__ ExArgs a) {
+  using X = Xt<QT>;
+  constexpr int ROWS = X::kRows, NS = X::kStages, ROTATORS = 32 * X::kRotWarps;
+  extern __shared__ __align__(1024) unsigned char xt_smem[];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const uint32_t sbase = smem_u32(xt_smem);
+  // (cos, cos, sin, sin) of the turn from one of a loader's keys to the next, two frequencies each
+  float* turn = reinterpret_cast<float*>(xt_smem + X::kTurnOff);
+  ExScratch<X::kSegs>& sc = *reinterpret_cast<ExScratch<X::kSegs>*>(xt_smem + X::kScratchOff);
+  if (tid < 64) {
+    float sn, cs;
+    rot_sincos(static_cast<float>(ROTATORS / 8), a.rot.hi[tid], a.rot.lo[tid], &sn, &cs);
+    turn[(tid >> 1) * 4 + (tid & 1)] = cs;
+    turn[(tid >> 1) * 4 + (tid & 1) + 2] = sn;
+  }
 
   pdl_wait();
   pdl_trigger();
-  const int kvh = blockIdx.x % a.num_kv_heads, slot = blockIdx.x / a.num_kv_heads;
-  const ExItem it = ex_find<ROWS, kPdTile, kExThreads>(a, slot, blockIdx.x == 0);
-  if (it.b < 0) return;
+  if ((sbase & 1023u) != 0) {   // the swizzled layouts need the 1024-byte alignment asked for above
+    if (tid == 0 && a.err != nullptr) atomicOr(a.err, kErrBadPointer);
+    return;
+  }
+  const int kvh = blockIdx.x % a.num_kv_heads, share = blockIdx.x / a.num_kv_heads;
+  const long long per = ex_share<ROWS, X::kThreads>(a, blockIdx.x == 0, sc);
+  if (tid == 0) {
+    sc.begin = share * per;
+    sc.end = sc.begin + per;
+  }
+  __syncthreads();
   const int gmask = (1 << a.lg) - 1;
   const int Nq = a.num_kv_heads << a.lg, P = a.page_size;
-  const int row0 = it.tile * ROWS;                    // of the request's n * G rows
-  const int nrows = min(ROWS, (it.n << a.lg) - row0);
-  const int pos0 = it.len - it.n;                     // position of the request's first new token
-  const int pos_first = pos0 + (row0 >> a.lg), pos_last = pos0 + ((row0 + nrows - 1) >> a.lg);
-  const int nkeys = max(0, min(it.len, pos_last + 1));
-  const int ntiles = (nkeys + kPdTile - 1) / kPdTile;
-  const int tile0 = it.range * it.per;
-  const int ntl = max(0, min(ntiles, tile0 + it.per) - tile0);                      // tiles of this CTA
-  const int ntw = ntl > warp ? (ntl - warp + kPdWarps - 1) / kPdWarps : 0;          // tiles of this warp
 
-  // ---- the rotated, pre-scaled queries, the B operand: [ROWS][128] in shared memory ----
-  {
-    const int d0 = (tid & 15) * 4;            // dims d0..d0+3 and their partners d0+64..
-    const float qscale = 1.4426950408889634f * rsqrtf(static_cast<float>(kPdDim));   // log2(e) / sqrt(d)
-    uint2 uo[NT], up[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int r = (tid >> 4) + 8 * i;
-      uo[i] = up[i] = make_uint2(0u, 0u);
-      if (r < nrows) {
-        const int rr = row0 + r;
-        const T* qp = static_cast<const T*>(a.q) + (static_cast<size_t>(it.qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim + d0;
-        uo[i] = __ldg(reinterpret_cast<const uint2*>(qp));
-        up[i] = __ldg(reinterpret_cast<const uint2*>(qp + 64));
-      }
+  const uint32_t qs = sbase, ks0 = sbase + X::kKOff, vs0 = sbase + X::kVOff, bars = sbase + X::kBarOff;
+  const uint32_t k_raw = bars, k_full = k_raw + NS * 8, k_empty = k_full + NS * 8, v_full = k_empty + NS * 8, v_empty = v_full + NS * 8;
+  // two each, used by alternate tiles: a softmax warp may be a tile ahead of another, and looks at the completion of a tile
+  // after it has handed on the next
+  const uint32_t s_full = v_empty + NS * 8, p_full = s_full + 16, o_done = s_full + 32;
+  const uint32_t q_full = s_full + 48, tmem_slot = s_full + 56;
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(xt_smem + (tmem_slot - sbase));
+  // roles: softmax warps w < 8 with w mod 4 < QT; of the others, in the order of their numbers, the rotators, a loader of K,
+  // one of V, the issuers of S and of O
+  const bool softmax = warp < 8 && (warp & 3) < QT;
+  const int other = warp - (warp < 4 ? min(warp, QT) : warp < 8 ? QT + min(warp - 4, QT) : 2 * QT);
+  const int role = softmax ? -1 : max(0, other - X::kRotWarps + 1);   // 0 rotator, 1 K, 2 V, 3 S, 4 O
+
+  ex_layout<ROWS, X::kThreads>(a, sc.begin, per, a.cuts == nullptr ? nullptr : a.cuts + blockIdx.x, sc);
+  if (sc.count == 0) return;   // nothing left for this share (uniform over the CTA)
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(k_raw + i * 8, 32);
+      mbar_init(k_full + i * 8, ROTATORS);
+      mbar_init(k_empty + i * 8, 1);
+      mbar_init(v_full + i * 8, 32);
+      mbar_init(v_empty + i * 8, 1);
     }
-    // (the table is in shared memory since the barriers of ex_find)
-    if (tid < 64) {
-      float sn, cs;
-      float* r = rot + (tid >> 1) * 4 + (tid & 1);
-      rot_sincos(static_cast<float>(kPdStep), freq[tid], freq[64 + tid], &sn, &cs);
-      r[0] = cs;
-      r[2] = sn;
-      rot_sincos(8.0f, freq[tid], freq[64 + tid], &sn, &cs);
-      r[128] = cs;
-      r[130] = sn;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i * 8, 1);
+      mbar_init(p_full + i * 8, 64 * QT);
+      mbar_init(o_done + i * 8, 1);   // also: the S buffer, where P lives, is free
     }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int r = (tid >> 4) + 8 * i;
-      const float pos = static_cast<float>(pos0 + ((row0 + r) >> a.lg));
-      const float2 o0 = unpack2<T>(uo[i].x), o1 = unpack2<T>(uo[i].y), q0 = unpack2<T>(up[i].x), q1 = unpack2<T>(up[i].y);
-      const float own[4] = {o0.x, o0.y, o1.x, o1.y}, par[4] = {q0.x, q0.y, q1.x, q1.y};
-      float ro[4], rp[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float sn, cs;
-        rot_sincos(pos, freq[d0 + k], freq[64 + d0 + k], &sn, &cs);
-        ro[k] = (own[k] * cs - par[k] * sn) * qscale;
-        rp[k] = (par[k] * cs + own[k] * sn) * qscale;
-      }
-      const int c_own = d0 >> 3, c_par = (d0 + 64) >> 3;
-      const uint32_t off = (d0 & 7) * 2;
-      asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(qs + r * 256 + ((c_own ^ (r & 7)) << 4) + off),
-                   "r"(pack2<T>(ro[0], ro[1])), "r"(pack2<T>(ro[2], ro[3])) : "memory");
-      asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(qs + r * 256 + ((c_par ^ (r & 7)) << 4) + off),
-                   "r"(pack2<T>(rp[0], rp[1])), "r"(pack2<T>(rp[2], rp[3])) : "memory");
-    }
+    mbar_init(q_full, 64 * QT);
+    fence_mbar_init();
   }
+  if (role == 3) {
+    tc_alloc(tmem_slot, kXtTmemCols);
+    tc_relinquish();
+  }
+  tc_fence_before();
   __syncthreads();
-  // B operand of k step ks (dimensions 16 ks ..) and of its partner ks + 4, rows 8 nt + g
-  const uint32_t q_row = (lane & 7) * 256;
-  const int q_chunk = ((lane >> 3) & 1) + ((lane >> 4) << 3);
-  auto load_q = [&](int nt, int ks, uint32_t (&f)[4]) {
-    ldsm_x4(f, qs + nt * 2048 + q_row + (((q_chunk + 2 * ks) ^ (lane & 7)) << 4));
-  };
-  uint32_t qf[NT == 1 ? 4 : 1][4];   // one column tile: kept in registers
-  if (NT == 1) {
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) load_q(0, ks, qf[NT == 1 ? ks : 0]);
-  }
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot_ptr;
+  bool dead = false;
+  int g = 0, gs = 0;   // tiles and row tiles so far, of the warp's role
 
-  // ---- this warp's ring and its loader ----
-  const uint32_t ring = sbase + warp * kPdWarpRing;
-  const size_t head_off = (static_cast<size_t>(a.layer_idx) * 2 * a.num_kv_heads + kvh) * P * kPdDim;
-  const size_t kv_delta = static_cast<size_t>(a.num_kv_heads) * P * kPdDim;
-  bool bad_ptr = false;
-  const int lp = 31 - __clz(P);   // the page size is a power of two (checked by the host)
-  // The two halves of a tile (keys 0-7 and 8-15) each lie inside one page.  Their addresses are looked up one tile ahead, so
-  // that the loads of the page table never sit in front of the copies.
-  const T* half_ptr[2] = {nullptr, nullptr};
-  auto lookup = [&](int j) {
-    half_ptr[0] = half_ptr[1] = nullptr;
-    if (j < ntw) {
-      const int key0 = (tile0 + warp + j * kPdWarps) * kPdTile;
+  for (;;) {
+    const int count = sc.count;
+    if (role == 0) {
+      // ---------------- rotators: thread = (chunk c of 8 dims and its partner, every STEP-th key) ----------------
+      constexpr int STEP = ROTATORS / 8, KPT = kXtKeys / STEP;   // keys of a thread per tile
+      const int rt = other * 32 + lane, c = rt & 7, kr = rt >> 3;
+      const ulonglong2* my_turn = reinterpret_cast<const ulonglong2*>(turn) + c * 4;
+      uint64_t cc[4] = {}, ss[4] = {};   // cosines and sines of key kr + STEP i, two frequencies each
+      for (int seg = 0; seg < count; ++seg) {
+        const int tile0 = sc.seg[seg].tile0, ntiles = sc.seg[seg].ntiles;
+        for (int j = 0; j < ntiles; ++j, ++g) {
+          if (j % kXtReseed == 0) {
+            const float pos = static_cast<float>((tile0 + j) * kXtKeys + kr);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int gk = key0 + 8 * h;
-        if (gk < nkeys) {
-          const T* page = static_cast<const T*>(a.kv_ptrs[it.p0 + (gk >> lp)]);
-          if (page == nullptr || (reinterpret_cast<uintptr_t>(page) & 15) != 0) bad_ptr = true;
-          else half_ptr[h] = page + head_off + static_cast<size_t>(gk & (P - 1)) * kPdDim;
-        }
-      }
-    }
-  };
-  // lane l copies chunk l & 15 of the keys 2 k + (l >> 4); chunk c of key e sits at slot c ^ (e & 7)
-  const int cch = lane & 15, ckey = lane >> 4;
-  const uint32_t dst_row = ckey * 256;
-  auto issue = [&](int j) {   // j-th tile of this warp; its addresses were looked up before
-    if (j < ntw) {
-      const int key0 = (tile0 + warp + j * kPdWarps) * kPdTile;
-      const uint32_t kst = ring + (j % kPdStages) * (2 * kPdTileBytes) + dst_row;
-      const int valid = nkeys - key0 - ckey;   // key 2 k of this lane exists if 2 k < valid
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool have = half_ptr[h] != nullptr;
-        const T* src = have ? half_ptr[h] + ckey * kPdDim + cch * 8 : static_cast<const T*>(a.q);
-        const T* vsrc = have ? src + kv_delta : src;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool ok = have && 8 * h + 2 * k < valid;                    // keys past the end read as zeros
-          const int step = ok ? 2 * k * kPdDim : 0;
-          const uint32_t dst = kst + (8 * h + 2 * k) * 256 + ((cch ^ (2 * k + ckey)) << 4);
-          cp_async16(dst, src + step, ok);
-          cp_async16(dst + kPdTileBytes, vsrc + step, ok);
-        }
-      }
-    }
-    cp_async_commit();
-    lookup(j + 1);
-  };
-  lookup(0);
-#pragma unroll
-  for (int j = 0; j < kPdStages - 1; ++j) issue(j);
-
-  // cosines and sines of key g of the tile: pair p = 2 ks + h holds the frequencies 16 ks + 8 h + 2 t and the next
-  uint64_t cc[8], ss[8];
-  float m_run[NT][2], l_run[NT][2];          // rows 8 nt + 2 t and the next
-  float o[NT][8][4];                         // dims 16 i + g and + 8 of those rows
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m_run[n][0] = m_run[n][1] = -INFINITY;
-    l_run[n][0] = l_run[n][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-  }
-  const int lm = lane >> 3, lr = lane & 7;
-  const uint32_t k_row = ((lm & 1) * 8 + lr) * 256, k_x = ((lm >> 1) ^ lr) << 4;             // matrices: key half, dim half
-  const uint32_t v_row = kPdTileBytes + ((lm >> 1) * 8 + lr) * 256, v_x = ((lm & 1) ^ lr) << 4;  // dim half, key half
-
-  for (int j = 0; j < ntw; ++j) {
-    issue(j + kPdStages - 1);
-    const int key0 = (tile0 + warp + j * kPdWarps) * kPdTile;
-    if (j % kPdReseed == 0) {
-      const float pos = static_cast<float>(key0 + g);
-#pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        float s0, s1, c0, c1;
-        const int f = 8 * p + 2 * t;
-        rot_sincos(pos, freq[f], freq[64 + f], &s0, &c0);
-        rot_sincos(pos, freq[f + 1], freq[64 + f + 1], &s1, &c1);
-        cc[p] = pack_f32x2(c0, c1);
-        ss[p] = pack_f32x2(s0, s1);
-      }
-    }
-    cp_async_wait<kPdStages - 1>();
-    __syncwarp();
-    const uint32_t kst = ring + (j % kPdStages) * (2 * kPdTileBytes);
-    // S^T = K . Q^T with the keys rotated on the way
-    float sc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t own[4], par[4];
-      const uint32_t ka = kst + k_row + (k_x ^ (ks << 5));
-      ldsm_x4(own, ka);
-      ldsm_x4(par, ka + 128);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int p = 2 * ks + h;
-        const ulonglong2 t8 = *reinterpret_cast<const ulonglong2*>(rot + 128 + (4 * p + t) * 4);
-        const ulonglong2 tw = *reinterpret_cast<const ulonglong2*>(rot + (4 * p + t) * 4);
-        uint64_t c = cc[p], s = ss[p];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {   // key g, then key g + 8
-          const float2 x = unpack2<T>(own[2 * h + e]), y = unpack2<T>(par[2 * h + e]);
-          const uint64_t ko = pack_f32x2(x.x, x.y), kp = pack_f32x2(y.x, y.y);
-          float a0, a1, b0, b1;
-          unpack_f32x2(fma_f32x2(ko, c, mul_f32x2(kp, s ^ 0x8000000080000000ull)), a0, a1);   // ko c - kp s
-          unpack_f32x2(fma_f32x2(kp, c, mul_f32x2(ko, s)), b0, b1);                           // kp c + ko s
-          own[2 * h + e] = pack2<T>(a0, a1);
-          par[2 * h + e] = pack2<T>(b0, b1);
-          if (e == 0) turn_f32x2(c, s, t8.x, t8.y);
-        }
-        turn_f32x2(cc[p], ss[p], tw.x, tw.y);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        uint32_t f[4];
-        if (NT == 1) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[i] = qf[NT == 1 ? ks : 0][i];
-        } else {
-          load_q(n, ks, f);
-        }
-        mma16816<T>(sc[n], own, f[0], f[1]);
-        mma16816<T>(sc[n], par, f[2], f[3]);
-      }
-    }
-    // running softmax: keys g and g + 8 of rows 8 n + 2 t and the next
-    if (key0 + kPdTile - 1 > pos_first) {   // a row of the tile does not see all of these keys
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = row0 + 8 * n + 2 * t + (i & 1);
-          if (key0 + g + (i >> 1) * 8 > min(pos0 + (row >> a.lg), pos_last)) sc[n][i] = -INFINITY;
-        }
-    }
-    bool up = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      up |= fmaxf(sc[n][0], sc[n][2]) > m_run[n][0] || fmaxf(sc[n][1], sc[n][3]) > m_run[n][1];
-    if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float mx = fmaxf(sc[n][q], sc[n][q + 2]);
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const float mn = fmaxf(m_run[n][q], mx);
-          const float rescale = mn == -INFINITY ? 1.0f : exp2f(m_run[n][q] - mn);   // exp2f(-inf) = 0 on the first key
-          m_run[n][q] = mn;
-          l_run[n][q] *= rescale;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            o[n][i][q] *= rescale;
-            o[n][i][q + 2] *= rescale;
+            for (int k = 0; k < 4; ++k) {
+              float s0, sx, c0, cx;
+              rot_sincos(pos, a.rot.hi[c * 8 + 2 * k], a.rot.lo[c * 8 + 2 * k], &s0, &c0);
+              rot_sincos(pos, a.rot.hi[c * 8 + 2 * k + 1], a.rot.lo[c * 8 + 2 * k + 1], &sx, &cx);
+              cc[k] = pack_f32x2(c0, cx);
+              ss[k] = pack_f32x2(s0, sx);
+            }
           }
-        }
-    }
-    uint32_t pb[NT][2];
+          const int st = g % NS;
+          pf_wait_role(k_raw + st * 8, (g / NS) & 1, a.err, dead);
+          // row kr of a panel; rows STEP further on are swizzled alike
+          uint32_t at = ks0 + st * kXtTileBytes + kr * 128 + ((c ^ (kr & 7)) << 4);
+#pragma unroll 1
+          for (int i0 = 0; i0 < KPT; i0 += 2, at += 2 * STEP * 128) {   // two keys at a time: both are read before either is written
+            uint32_t own[2][4], par[2][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float pr[4];
+            for (int i = 0; i < 2; ++i) {
+              lds128(at + i * (STEP * 128), own[i]);
+              lds128(at + i * (STEP * 128) + kXtPanel, par[i]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const ulonglong2 t1 = my_turn[k];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float2 x = unpack2<T>(own[i][k]), y = unpack2<T>(par[i][k]);
+                const uint64_t ko = pack_f32x2(x.x, x.y), kq = pack_f32x2(y.x, y.y);
+                const uint64_t ns = ss[k] ^ 0x8000000080000000ull;
+                float a0, a1, b0, b1;
+                unpack_f32x2(fma_f32x2(ko, cc[k], mul_f32x2(kq, ns)), a0, a1);      // own c - partner s
+                unpack_f32x2(fma_f32x2(kq, cc[k], mul_f32x2(ko, ss[k])), b0, b1);   // partner c + own s
+                own[i][k] = pack2<T>(a0, a1);
+                par[i][k] = pack2<T>(b0, b1);
+                // the next of the thread's keys; after the last of them the tile's 64 keys are passed
+                const uint64_t n = fma_f32x2(cc[k], t1.x, mul_f32x2(ns, t1.y));
+                ss[k] = fma_f32x2(ss[k], t1.x, mul_f32x2(cc[k], t1.y));
+                cc[k] = n;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              sts128(at + i * (STEP * 128), own[i]);
+              sts128(at + i * (STEP * 128) + kXtPanel, par[i]);
+            }
+          }
+          fence_proxy_async();   // the products read through the async proxy
+          mbar_arrive(k_full + st * 8);
+        }
+      }
+    } else if (role == 1 || role == 2) {
+      // ---------------- loaders: a warp copies a tile, a lane chunk lane & 15 of the keys 2 i + (lane >> 4) ----------------
+      const uint32_t ring = role == 1 ? ks0 : vs0, full = role == 1 ? k_raw : v_full, empty = role == 1 ? k_empty : v_empty;
+      const int lp = 31 - __clz(P);   // the page size is a power of two (checked by the host)
+      const uint32_t head_off =
+          static_cast<uint32_t>(((a.layer_idx * 2 + role - 1) * a.num_kv_heads + kvh) * P) * 256u;   // bytes
+      const uint32_t lane_off = (lane >> 4) * 256 + (lane & 15) * 16;
+      uint32_t dst[4];   // of the keys 2 i + (lane >> 4) of a group of eight: panel, row, swizzled chunk
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float m = m_run[n][i & 1];
-        pr[i] = exp2f(sc[n][i] - (m == -INFINITY ? 0.f : m));   // a row that has seen no key yet: zeros
+        const int row = 2 * i + (lane >> 4);
+        dst[i] = ring + ((lane & 8) ? kXtPanel : 0) + row * 128 + (((lane & 7) ^ row) << 4);
       }
-      l_run[n][0] += pr[0] + pr[2];
-      l_run[n][1] += pr[1] + pr[3];
-      pb[n][0] = movm_t(pack2<T>(pr[0], pr[1]));
-      pb[n][1] = movm_t(pack2<T>(pr[2], pr[3]));
-    }
-    // O^T += V^T . P^T ; P comes as [key][rows] and was transposed into the B operand
+      bool bad_ptr = false;
+      // eight keys lie in one page: lane e looks after the keys 8 e .. 8 e + 7 of the tile, a tile ahead of the copies
+      const int e8 = (lane & 7) * 8;
+      auto entry = [&](const ExSeg& s, int tile) {
+        const int key = tile * kXtKeys + e8;
+        return load_if(a.kv_ptrs + s.p0 + (key >> lp), key < s.nkeys);
+      };
+      int seg = 0;
+      while (seg < count && sc.seg[seg].ntiles == 0) ++seg;
+      uint64_t page = seg < count ? entry(sc.seg[seg], sc.seg[seg].tile0) : 0;
+      while (seg < count) {
+        const int tile0 = sc.seg[seg].tile0, ntiles = sc.seg[seg].ntiles, nkeys = sc.seg[seg].nkeys;
+        int next = seg + 1;
+        while (next < count && sc.seg[next].ntiles == 0) ++next;
+        for (int j = 0; j < ntiles; ++j, ++g) {
+          const int key0 = (tile0 + j) * kXtKeys;
+          const bool ok = page != 0 && (page & 15) == 0;
+          bad_ptr |= key0 + e8 < nkeys && !ok;
+          const uint64_t base = page + head_off + ((key0 + e8) & (P - 1)) * 256u;
+          const bool whole = __all_sync(0xffffffffu, ok) && key0 + kXtKeys <= nkeys;
+          const uint64_t mine = ok ? base : 0;
+          page = j + 1 < ntiles ? entry(sc.seg[seg], tile0 + j + 1) : next < count ? entry(sc.seg[next], sc.seg[next].tile0) : 0;
+          const int st = g % NS;
+          if (g >= NS) pf_wait_role(empty + st * 8, (g / NS - 1) & 1, a.err, dead);
+          if (dead) break;
+          const uint32_t off = st * kXtTileBytes;
+          if (whole) {
+            auto src = [&](int e) { return __shfl_sync(0xffffffffu, mine, e) + lane_off; };
+            copy_eight<0>(dst, off, src(0));
+            copy_eight<1>(dst, off, src(1));
+            copy_eight<2>(dst, off, src(2));
+            copy_eight<3>(dst, off, src(3));
+            copy_eight<4>(dst, off, src(4));
+            copy_eight<5>(dst, off, src(5));
+            copy_eight<6>(dst, off, src(6));
+            copy_eight<7>(dst, off, src(7));
+          } else {
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) {   // keys that do not exist read as zeros
+              const uint64_t src = __shfl_sync(0xffffffffu, mine, e) + lane_off;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t vf[4];
-      ldsm_x4_t(vf, kst + v_row + ((i >> 2) << 7) + (v_x ^ ((i & 3) << 5)));
+              for (int i = 0; i < 4; ++i) {
+                const bool have = src != lane_off && key0 + 8 * e + 2 * i + (lane >> 4) < nkeys;
+                cp_async16(dst[i] + off + e * 1024, have ? reinterpret_cast<const void*>(src + i * 512) : a.q, have);
+              }
+            }
+          }
+          cp_async_arrive(full + st * 8);   // when this lane's copies have landed
+        }
+        if (dead) break;
+        seg = next;
+      }
+      cp_async_wait<0>();
+      if (__any_sync(0xffffffffu, bad_ptr) && lane == 0 && a.err != nullptr) atomicOr(a.err, kErrBadPointer);
+    } else if (role == 3) {
+      // ---------------- issuer of S = Q . K^T: runs up to two tiles ahead of the softmax ----------------
+      if (lane == 0) {
+        const uint32_t idesc_s = tc_idesc<T>(kXtKeys, false);
+        const uint64_t qdesc = desc_kmajor(qs), kdesc = desc_kmajor(ks0);   // (addresses are added below: no field overflows)
+        for (int seg = 0; seg < count; ++seg) {
+          const int ntiles = sc.seg[seg].ntiles;
+          if (ntiles == 0) continue;
+          pf_wait_role(q_full, gs & 1, a.err, dead);
+          for (int j = 0; j < ntiles; ++j, ++g) {
+            const int st = g % NS, sb = g & 1;
+            pf_wait_role(k_full + st * 8, (g / NS) & 1, a.err, dead);
+            if (g >= 2) pf_wait_role(o_done + sb * 8, ((g >> 1) - 1) & 1, a.err, dead);   // P . V has read this S buffer
+            tc_fence_after();
+            if (!dead) {
+              const uint64_t kd = kdesc + st * (kXtTileBytes >> 4);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma16816<T>(o[n][i], vf, pb[n][0], pb[n][1]);
-    }
-    __syncwarp();   // the stage is free for the copy issued in the next iteration
-  }
-  cp_async_wait<0>();
-  if (__any_sync(0xffffffffu, bad_ptr) && lane == 0 && a.err != nullptr) atomicOr(a.err, kErrBadPointer);
+              for (int kk = 0; kk < 8; ++kk)
+                tc_mma(tmem + sb * kXtKeys, qdesc + (((kk >> 2) * X::kQPanel + (kk & 3) * 32) >> 4),
+                       kd + (((kk >> 2) * kXtPanel + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+            }
+            tc_commit(s_full + sb * 8);
+            tc_commit(k_empty + st * 8);
+          }
+          ++gs;
+        }
+      }
+    } else if (role == 4) {
+      // ---------------- issuer of O += P . V ----------------
+      if (lane == 0) {
+        const uint32_t idesc_o = tc_idesc<T>(kPdDim, true);
+        const uint64_t vdesc = desc_mnmajor(vs0, kXtPanel);
+        for (int seg = 0; seg < count; ++seg) {
+          const int ntiles = sc.seg[seg].ntiles;
+          for (int j = 0; j < ntiles; ++j, ++g) {
+            const int st = g % NS, sb = g & 1;
+            pf_wait_role(v_full + st * 8, (g / NS) & 1, a.err, dead);
+            fence_proxy_async();   // V came by the loader's ordinary copies
+            pf_wait_role(p_full + sb * 8, (g >> 1) & 1, a.err, dead);
+            tc_fence_after();
+            if (!dead) {
+              const uint64_t vd = vdesc + st * (kXtTileBytes >> 4);
+              const uint32_t pa = tmem + sb * kXtKeys + kXtHalf / 2;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+              for (int kk = 0; kk < kXtKeys / 16; ++kk)   // keys 16 kk .. 16 kk + 15: eight columns in the upper half of the
+                                                          // columns of the thread that made them
+                tc_mma_ts(tmem + kXtOCol, pa + (kk >> 1) * kXtHalf + (kk & 1) * 8, vd + kk * (2048 >> 4), idesc_o,
+                          (j > 0 || kk > 0) ? 1u : 0u);
+            }
+            tc_commit(o_done + sb * 8);
+            tc_commit(v_empty + st * 8);
+          }
+        }
+      }
+    } else {
+      // ---------------- softmax warps: thread = (row, half of the columns) ----------------
+      // Warps w and w + 4 (w < QT) hold the same 32 rows: the first takes columns 0-31 of a tile of S and 0-63 of O, the
+      // second the rest.  The two threads of a row agree on its maximum through tensor memory, as in the prefill kernel.
+      const int half = warp >> 2;
+      const int wq = warp & 3;
+      const int row = wq * 32 + lane;
+      const uint32_t my_tmem = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+      const uint32_t o_tmem = my_tmem + kXtOCol + half * 64;
+      for (int seg = 0; seg < count; ++seg) {
+        const ExSeg s = sc.seg[seg];
+        if (s.ntiles == 0) continue;
+        const int rr = s.row0 + row;
+        // rows past the end behave like the last one
+        const int my_pos = s.pos0 + (min(rr, s.row0 + s.nrows - 1) >> a.lg);
+        // ---- the rotated, pre-scaled queries: A operand, K-major.  16 threads per row ----
+        {
+          const int qt = (half * QT + wq) * 32 + lane;
+          const int d0 = (qt & 15) * 4;
+          constexpr int PASS = 4 * QT;   // rows per pass
+          const float qscale = 1.4426950408889634f * rsqrtf(static_cast<float>(kPdDim));   // log2(e) / sqrt(d)
+          uint2 uo[8], up[8];
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+          for (int i = 0; i < 8; ++i) {
+            const int r = (qt >> 4) + PASS * i;
+            uo[i] = up[i] = make_uint2(0u, 0u);
+            if (r < s.nrows) {
+              const T* qp = static_cast<const T*>(a.q) +
+                            (static_cast<size_t>(s.qo0 + ((s.row0 + r) >> a.lg)) * Nq + (kvh << a.lg) + ((s.row0 + r) & gmask)) *
+                                kPdDim + d0;
+              uo[i] = __ldg(reinterpret_cast<const uint2*>(qp));
+              up[i] = __ldg(reinterpret_cast<const uint2*>(qp + 64));
+            }
+          }
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) l_run[n][q] += __shfl_xor_sync(0xffffffffu, l_run[n][q], d);
+          for (int i = 0; i < 8; ++i) {
+            const int r = (qt >> 4) + PASS * i;
+            const float pos = static_cast<float>(s.pos0 + ((s.row0 + r) >> a.lg));
+            const float2 o0 = unpack2<T>(uo[i].x), o1 = unpack2<T>(uo[i].y), q0 = unpack2<T>(up[i].x), q1 = unpack2<T>(up[i].y);
+            const float own[4] = {o0.x, o0.y, o1.x, o1.y}, par[4] = {q0.x, q0.y, q1.x, q1.y};
+            float ro[4], rp[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float sn, cs;
+              rot_sincos(pos, a.rot.hi[d0 + k], a.rot.lo[d0 + k], &sn, &cs);
+              ro[k] = (own[k] * cs - par[k] * sn) * qscale;
+              rp[k] = (par[k] * cs + own[k] * sn) * qscale;
+            }
+            const uint32_t addr = qs + r * 128 + (((d0 >> 3) ^ (r & 7)) << 4) + (d0 & 7) * 2;
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(addr), "r"(pack2<T>(ro[0], ro[1])), "r"(pack2<T>(ro[2], ro[3]))
+                         : "memory");
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(addr + X::kQPanel), "r"(pack2<T>(rp[0], rp[1])),
+                         "r"(pack2<T>(rp[2], rp[3])) : "memory");
+          }
+          fence_proxy_async();   // the products read Q through the async proxy
+          mbar_arrive(q_full);
+        }
+        if (wq * 32 >= s.nrows) {   // no row of the tile: hands on what the others make
+          for (int j = 0; j < s.ntiles; ++j, ++g) {
+            pf_wait_role(s_full + (g & 1) * 8, (g >> 1) & 1, a.err, dead);
+            mbar_arrive(p_full + (g & 1) * 8);
+          }
+          continue;
+        }
 
-  // ---- merge the warps in warp order, eight rows at a time: per (warp, row) m, l, 2 unused, o[128]; thread = dim ----
-  float* red = reinterpret_cast<float*>(ex_smem_buf);
-  constexpr int REC = kPdRec;
+        float m_ref = -INFINITY;
+        uint64_t l2 = pack_f32x2(0.f, 0.f);   // this thread's share of the row sum, two lanes
+        for (int j = 0; j < s.ntiles; ++j, ++g) {
+          const int sb = g & 1;
+          pf_wait_role(s_full + sb * 8, (g >> 1) & 1, a.err, dead);
+          tc_fence_after();
+          const uint32_t my_s = my_tmem + sb * kXtKeys + half * kXtHalf;
+          const int lim = my_pos - (s.tile0 + j) * kXtKeys - half * kXtHalf;   // columns above lim are later keys
+          uint32_t sv[32];
+          tc_ld32(my_s, sv);
+          tc_wait_ld();
+          if (lim < 31) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    __syncthreads();   // the rings, then the previous eight rows, are done with
+            for (int i = 0; i < 32; ++i)
+              if (i > lim) sv[i] = __float_as_uint(-INFINITY);
+          }
+          float ma = max3(__uint_as_float(sv[0]), __uint_as_float(sv[1]), __uint_as_float(sv[2]));
+          float mb = max3(__uint_as_float(sv[3]), __uint_as_float(sv[4]), __uint_as_float(sv[5]));
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      float* r = red + (warp * 8 + 2 * t + q) * REC;
-      if (g == 0) {
-        r[0] = m_run[n][q];
-        r[1] = l_run[n][q];
-      }
+          for (int i = 6; i < 30; i += 4) {
+            ma = max3(ma, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+            mb = max3(mb, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
+          }
+          float mx = fmaxf(max3(ma, __uint_as_float(sv[30]), __uint_as_float(sv[31])), mb);
+          // exchange with the other half's thread: own maximum into the first column of the own half
+          tc_st1(my_s, __float_as_uint(mx));
+          tc_wait_st();
+          tc_fence_before();
+          pair_barrier(wq);
+          tc_fence_after();
+          mx = fmaxf(mx, __uint_as_float(tc_ld1(my_tmem + sb * kXtKeys + (half ^ 1) * kXtHalf)));
+          float rescale = 1.0f;
+          bool raise = false;
+          if (mx > m_ref + kPfRaise || m_ref == -INFINITY) {   // (-inf + 8 = -inf: the first visible key always raises)
+            if (mx != -INFINITY) {
+              raise = m_ref != -INFINITY;
+              rescale = exp2f(m_ref - mx);   // 0 when nothing was accumulated yet
+              m_ref = mx;
+            }
+          }
+          const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
+          const uint64_t nm2 = pack_f32x2(nm, nm);
+          uint64_t sum2 = pack_f32x2(0.f, 0.f);
+          uint32_t pw[kXtHalf / 2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        r[4 + 16 * i + g] = o[n][i][q];
-        r[4 + 16 * i + 8 + g] = o[n][i][q + 2];
+          for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            unpack_f32x2(add_f32x2(pack_f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), nm2), x0, x1);
+            const float e0 = exp2f(x0), e1 = exp2f(x1);
+            sum2 = add_f32x2(sum2, pack_f32x2(e0, e1));
+            pw[i >> 1] = pack2<T>(e0, e1);
+          }
+          l2 = add_f32x2(mul_f32x2(l2, pack_f32x2(rescale, rescale)), sum2);
+          bool waited = j == 0;
+          auto wait_prev = [&]() {   // P . V of the previous tile has completed: O is stable
+            if (!waited) {
+              pf_wait_role(o_done + (sb ^ 1) * 8, ((g - 1) >> 1) & 1, a.err, dead);
+              tc_fence_after();
+              waited = true;
+            }
+          };
+          if (j > 0 && __any_sync(0xffffffffu, raise)) {
+            wait_prev();
+#pragma unroll 1
+            for (int q = 0; q < 2; ++q) {
+              uint32_t ov[32];
+              tc_ld32(o_tmem + q * 32, ov);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * rescale);
+              tc_st32(o_tmem + q * 32, ov);
+            }
+            tc_wait_st();
+          }
+          // P overwrites the upper half of the S columns this thread has read (the lower half keeps the exchanged
+          // maximum); the other thread of the row has read its own columns before the exchange
+          tc_st16(my_s + kXtHalf / 2, pw);
+          tc_wait_st();
+          tc_fence_before();
+          mbar_arrive(p_full + sb * 8);
+          wait_prev();   // every phase of the barrier is consumed, so that its parity stays readable
+        }
+
+        // ---- the result O / l, or the state; the two halves' sums meet through tensor memory as the maxima did ----
+        pf_wait_role(o_done + ((g - 1) & 1) * 8, ((g - 1) >> 1) & 1, a.err, dead);
+        tc_fence_after();
+        float la, lb;
+        unpack_f32x2(l2, la, lb);
+        const float l_mine = la + lb;
+        tc_st1(my_tmem + half * kXtHalf, __float_as_uint(l_mine));   // S buffer 0: the next product waits for this warp's queries
+        tc_wait_st();
+        tc_fence_before();
+        pair_barrier(wq);
+        tc_fence_after();
+        const float l_run = l_mine + __uint_as_float(tc_ld1(my_tmem + (half ^ 1) * kXtHalf));
+        const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;   // no keys: zeros; a NaN stays one
+        T* orow = static_cast<T*>(a.o) + (static_cast<size_t>(s.qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim;
+        float* rec = a.partial + (((static_cast<size_t>(share) * 2 + max(s.part, 0)) * a.num_kv_heads + kvh) * ROWS + row) * kPdRec;
+        const bool write = row < s.nrows && !dead;
+        if (write && s.part >= 0 && half == 0) {
+          rec[0] = m_ref;
+          rec[1] = l_run;
+        }
+#pragma unroll 1
+        for (int q = 0; q < 2; ++q) {
+          uint32_t ov[32];
+          tc_ld32(o_tmem + q * 32, ov);
+          tc_wait_ld();
+          if (!write) continue;
+          if (s.part >= 0) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(rec + 4 + half * 64 + q * 32 + i) = make_uint4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float f[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(ov[i + k]) * inv;
+              *reinterpret_cast<uint4*>(orow + half * 64 + q * 32 + i) =
+                  make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+            }
+          }
+        }
+        tc_fence_before();   // the next row tile's products overwrite O after this warp has handed on a P
       }
     }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 8; ++h) {
-      const int row = 8 * n + h;
-      if (row >= nrows) break;
-      float m = -INFINITY, l = 0.f, acc = 0.f;
-#pragma unroll
-      for (int w = 0; w < kPdWarps; ++w) {
-        const float* r = red + (w * 8 + h) * REC;
-        if (r[1] != 0.f) m = fmaxf(m, r[0]);   // an empty state carries no information
-      }
-#pragma unroll
-      for (int w = 0; w < kPdWarps; ++w) {
-        const float* r = red + (w * 8 + h) * REC;
-        if (r[1] != 0.f) {
-          const float wt = exp2f(r[0] - m);
-          l += r[1] * wt;
-          acc += r[4 + tid] * wt;
-        }
-      }
-      if (it.ranges == 1) {
-        const int rr = row0 + row;
-        static_cast<T*>(a.o)[(static_cast<size_t>(it.qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim + tid] =
-            static_cast<T>(l == 0.f ? 0.f : acc * (1.0f / l));   // no keys: zeros; a NaN stays one
-      } else {
-        float* r = a.partial + ((static_cast<size_t>(slot) * a.num_kv_heads + kvh) * ROWS + row) * REC;
-        if (tid == 0) {
-          r[0] = m;
-          r[1] = l;
-        }
-        r[4 + tid] = acc;
-      }
-    }
+    if (sc.next >= sc.end) break;
+    const long long w0 = sc.next;
+    __syncthreads();   // everyone is done with this round's runs
+    ex_layout<ROWS, X::kThreads>(a, w0, 1, nullptr, sc);
+    if (sc.count == 0) break;
   }
+
+  // everyone is done with tensor memory: hand it back
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (role == 3) tc_dealloc(tmem, kXtTmemCols);
 }
 
-// Merges the parked states of tiles with several ranges, in range order.  The CTA of range r serves the tile's rows
-// r, r + ranges, ...; thread = dim.
-template <typename T, int ROWS, int KEYS>
-__global__ void __launch_bounds__(kExThreads) paged_extend_merge_kernel(const __grid_constant__ ExArgs a) {
-  // The index arrays were complete before the kernel in front started (it waited for them itself), so the search
-  // needs no wait; the parked states do.
-  const int kvh = blockIdx.x % a.num_kv_heads, slot = blockIdx.x / a.num_kv_heads;
-  const ExItem it = ex_find<ROWS, KEYS, kExThreads>(a, slot, false);
+// Merges the states of the row tiles that are cut, in the order of the keys.  grid: ((shares - 1) * Nkv, kXtMergeSplit); a
+// CTA stands for the cut at the start of a share and serves some of the rows of the tile that it goes through, a warp a row
+// at a time, a lane four dimensions.
+constexpr int kXtMergeThreads = 256;
+constexpr int kXtMergeSplit = 2;
+
+template <typename T, int QT>
+__global__ void __launch_bounds__(kXtMergeThreads) paged_extend_merge_kernel(const __grid_constant__ ExArgs a) {
+  constexpr int ROWS = Xt<QT>::kRows, WARPS = kXtMergeThreads / 32;
   pdl_wait();
   pdl_trigger();
-  if (it.b < 0 || it.ranges == 1) return;
-  const int gmask = (1 << a.lg) - 1;
-  const int Nq = a.num_kv_heads << a.lg;
-  const int row0 = it.tile * ROWS;
-  const int nrows = min(ROWS, (it.n << a.lg) - row0);
-  const int ranges = min(it.ranges, a.slots - it.slot0);   // (an unsound table may ask for more than there is)
-  const size_t next = static_cast<size_t>(a.num_kv_heads) * ROWS * kPdRec;
-  for (int row = it.range; row < nrows; row += it.ranges) {
-    const float* r = a.partial + ((static_cast<size_t>(it.slot0) * a.num_kv_heads + kvh) * ROWS + row) * kPdRec;
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    constexpr int U = 8;
-    for (int z0 = 0; z0 < ranges; z0 += U) {   // eight states are requested together
-      float mz[U], lz[U], oz[U];
+  const int kvh = blockIdx.x % a.num_kv_heads, share = blockIdx.x / a.num_kv_heads + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4* rec = reinterpret_cast<const int4*>(a.cuts + blockIdx.x + a.num_kv_heads);
+  const int4 c0 = __ldcg(rec), c1 = __ldcg(rec + 1);
+  const int qo0 = c0.x, row0 = c0.y, nrows = c0.z, first = c0.w, count = c1.x, shares = c1.y, part = c1.z;
+  const int gmask = (1 << a.lg) - 1, Nq = a.num_kv_heads << a.lg;
+  const size_t share_step = static_cast<size_t>(2) * a.num_kv_heads * ROWS * kPdRec;
+  for (int i = blockIdx.y * WARPS + warp; ; i += kXtMergeSplit * WARPS) {
+    const int row = i * shares + share - first - 1;
+    if (nrows == 0 || row >= nrows) break;
+    const float* base = a.partial + ((static_cast<size_t>(first) * 2 * a.num_kv_heads + kvh) * ROWS + row) * kPdRec;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int U = 4;
+    for (int z0 = 0; z0 < count; z0 += U) {   // four states are requested together
+      float2 ml[U];
+      float4 o[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        mz[u] = lz[u] = oz[u] = 0.f;
-        if (z0 + u < ranges) {
-          mz[u] = __ldcg(r + (z0 + u) * next);
-          lz[u] = __ldcg(r + (z0 + u) * next + 1);
-          oz[u] = __ldcg(r + (z0 + u) * next + 4 + threadIdx.x);
+        ml[u] = make_float2(0.f, 0.f);
+        o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (z0 + u < count) {
+          const float* r = base + (z0 + u) * share_step +
+                           (z0 + u == 0 && part ? static_cast<size_t>(a.num_kv_heads) * ROWS * kPdRec : 0);
+          ml[u] = __ldcg(reinterpret_cast<const float2*>(r));
+          o[u] = __ldcg(reinterpret_cast<const float4*>(r + 4) + lane);
         }
       }
       float mn = m;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (lz[u] != 0.f) mn = fmaxf(mn, mz[u]);
-      if (l != 0.f) {
-        const float wt = exp2f(m - mn);
-        l *= wt;
-        acc *= wt;
-      }
+        if (ml[u].y != 0.f) mn = fmaxf(mn, ml[u].x);   // an empty state carries no information
+      const float w0 = l != 0.f ? exp2f(m - mn) : 0.f;
       m = mn;
+      l *= w0;
+      acc.x *= w0; acc.y *= w0; acc.z *= w0; acc.w *= w0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (lz[u] != 0.f) {
-          const float wt = exp2f(mz[u] - m);
-          l += lz[u] * wt;
-          acc += oz[u] * wt;
+        if (ml[u].y != 0.f) {
+          const float wt = exp2f(ml[u].x - m);
+          l += ml[u].y * wt;
+          acc.x += o[u].x * wt; acc.y += o[u].y * wt; acc.z += o[u].z * wt; acc.w += o[u].w * wt;
         }
       }
     }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
     const int rr = row0 + row;
-    static_cast<T*>(a.o)[(static_cast<size_t>(it.qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim + threadIdx.x] =
-        static_cast<T>(l == 0.f ? 0.f : acc * (1.0f / l));
+    T* op = static_cast<T*>(a.o) + (static_cast<size_t>(qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim;
+    reinterpret_cast<uint2*>(op)[lane] = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
   }
 }
 

@@ -194,6 +194,7 @@ class GrowableTensor:
     def _flush(self) -> None:
         if not self._pending:
             return
+        refuse_capture(self._buf, "the first look at a cache's page table after it grew")
         length = self._len + len(self._pending)
         new = device_ints(self._pending, self._buf.dtype, self._buf.device)
         if self._len == 0:

@@ -152,7 +152,7 @@ def test_c_abi_refusals():
     L = cabi.lib
     ws = L.smlm_b200_batch_extend_workspace_bytes(2, 8, 64, 16, 32, 8)
     assert ws > 0 and L.smlm_b200_batch_extend_workspace_bytes(0, 8, 64, 16, 32, 8) == 0
-    assert L.smlm_b200_batch_extend_workspace_bytes(1, 4, 2, 16, 32, 8) == 0        # 32 keys: a single range
+    assert L.smlm_b200_batch_extend_workspace_bytes(1, 4, 2, 16, 300, 300) == 0     # a CTA per kv head: nothing is cut
 
     def ext(o=256, wsp=256, bytes_=ws, rows=8, pages=64, nq=32, hd=128, layer=0, P=16, theta=10000.0, dt=1, batch=2):
         return L.smlm_b200_batch_extend(o, 256, 256, 256, 256, 256, wsp, bytes_, None, batch, rows, pages, nq, 8, hd, 1, layer,
