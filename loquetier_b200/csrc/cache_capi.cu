@@ -76,29 +76,43 @@ inline int head_splits(int T, int heads) {
   return std::max(1, std::min(want, (heads + 3) / 4));
 }
 
+// the streams of queries and keys, a unit per warp
+void qk_streams(HeadNormArgs& a, int Nq, int Nk) {
+  const int heads[2] = {Nq, Nk};
+  for (int i = 0; i < 2; ++i) {
+    a.s[i].heads = heads[i];
+    a.s[i].splits = head_splits(a.T, heads[i]);
+    a.s[i].ctas = static_cast<int>((static_cast<long long>(a.T) * a.s[i].splits + kHnWarps - 1) / kHnWarps);
+  }
+}
+
+// the backward pass: as many CTAs as are resident at most, shared out by the numbers of heads
+void qk_bwd_streams(HeadNormArgs& a, int Nq, int Nk) {
+  qk_streams(a, Nq, Nk);
+  const int resident = 2 * kNumSMs;
+  const int k_most = std::max(1, static_cast<int>(static_cast<long long>(resident) * Nk / (Nq + Nk)));
+  a.s[1].ctas = std::min(a.s[1].ctas, k_most);
+  a.s[0].ctas = std::min(a.s[0].ctas, std::max(1, resident - k_most));
+}
+
 template <typename T>
 int launch_qk_fwd(const HeadNormArgs& a, cudaStream_t stream) {
-  const bool norm = a.wq != nullptr, rope = a.positions != nullptr;
-  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.T) * a.splits + kHnWarps - 1) / kHnWarps), 1, 1);
+  const bool norm = a.s[0].w != nullptr, rope = a.positions != nullptr;
+  const dim3 grid(a.s[0].ctas + a.s[1].ctas, 1, 1);
   if (norm) return rope ? launch(qk_norm_rope_kernel<T, true, true>, grid, kHnThreads, 1, 0, stream, a)
                         : launch(qk_norm_rope_kernel<T, true, false>, grid, kHnThreads, 1, 0, stream, a);
   return launch(qk_norm_rope_kernel<T, false, true>, grid, kHnThreads, 1, 0, stream, a);
 }
 
-inline int qk_bwd_grid(int T, int splits) {
-  const long long ctas = (static_cast<long long>(T) * splits + kHnWarps - 1) / kHnWarps;
-  return static_cast<int>(std::min<long long>(ctas, 2 * kNumSMs));
-}
-
 template <typename T>
 int launch_qk_bwd(const HeadNormArgs& a, void* dwq, void* dwk, cudaStream_t stream) {
-  const bool norm = a.wq != nullptr, rope = a.positions != nullptr;
-  const dim3 grid(qk_bwd_grid(a.T, a.splits), 1, 1);
+  const bool norm = a.s[0].w != nullptr, rope = a.positions != nullptr;
+  const dim3 grid(a.s[0].ctas + a.s[1].ctas, 1, 1);
   if (!norm) return launch(qk_norm_rope_bwd_kernel<T, false, true>, grid, kHnThreads, 1, 0, stream, a);
   const int rc = rope ? launch(qk_norm_rope_bwd_kernel<T, true, true>, grid, kHnThreads, 1, 0, stream, a)
                       : launch(qk_norm_rope_bwd_kernel<T, true, false>, grid, kHnThreads, 1, 0, stream, a);
   if (rc != SMLM_OK) return rc;
-  return launch(head_norm_dw_kernel<T>, dim3(2 * kPdDim / 8, 1, 1), 256, 1, 0, stream, dwq, dwk, a.partial,
+  return launch(head_norm_dw_kernel<T>, dim3(2 * kPdDim / 8, 1, 1), 256, 1, 0, stream, dwq, dwk, a.partial, a.s[0].ctas,
                 static_cast<int>(grid.x));
 }
 
@@ -230,10 +244,10 @@ int smlm_b200_qk_norm_rope(void* yq, void* yk, const void* q, const void* k, con
   if (yq == nullptr || yk == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
   if (!aligned16(yq) || !aligned16(yk)) return SMLM_ERR_MISALIGNED;
   HeadNormArgs a = {};
-  a.q = q; a.k = k; a.wq = wq; a.wk = wk; a.positions = positions; a.yq = yq; a.yk = yk;
-  a.q_stride = q_stride; a.k_stride = k_stride; a.T = T; a.Nq = num_qo_heads; a.Nk = num_kv_heads; a.pos64 = positions_64;
-  a.eps = eps;
-  a.splits = head_splits(T, std::max(num_qo_heads, num_kv_heads));
+  a.positions = positions; a.T = T; a.pos64 = positions_64; a.eps = eps;
+  a.s[0].x = q; a.s[0].w = wq; a.s[0].y = yq; a.s[0].stride = q_stride;
+  a.s[1].x = k; a.s[1].w = wk; a.s[1].y = yk; a.s[1].stride = k_stride;
+  qk_streams(a, num_qo_heads, num_kv_heads);
   if (positions != nullptr) a.rot = rot_table(rope_theta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == SMLM_F16 ? launch_qk_fwd<__half>(a, st) : launch_qk_fwd<__nv_bfloat16>(a, st);
@@ -241,8 +255,10 @@ int smlm_b200_qk_norm_rope(void* yq, void* yk, const void* q, const void* k, con
 
 size_t smlm_b200_qk_norm_rope_bwd_workspace_bytes(int T, int num_qo_heads, int num_kv_heads) {
   if (T <= 0 || num_qo_heads <= 0 || num_kv_heads <= 0) return 0;
-  return static_cast<size_t>(qk_bwd_grid(T, head_splits(T, std::max(num_qo_heads, num_kv_heads)))) * 2 * kPdDim *
-         sizeof(float);
+  HeadNormArgs a = {};
+  a.T = T;
+  qk_bwd_streams(a, num_qo_heads, num_kv_heads);
+  return static_cast<size_t>(a.s[0].ctas + a.s[1].ctas) * kPdDim * sizeof(float);
 }
 
 int smlm_b200_qk_norm_rope_bwd(void* dq, void* dk, void* dwq, void* dwk, const void* gq, const void* gk, const void* q,
@@ -264,11 +280,10 @@ int smlm_b200_qk_norm_rope_bwd(void* dq, void* dk, void* dwq, void* dwk, const v
     if (!aligned16(workspace)) return SMLM_ERR_MISALIGNED;
   }
   HeadNormArgs a = {};
-  a.q = q; a.k = k; a.wq = wq; a.wk = wk; a.positions = positions; a.yq = dq; a.yk = dk; a.gq = gq; a.gk = gk;
-  a.partial = static_cast<float*>(workspace);
-  a.q_stride = q_stride; a.k_stride = k_stride; a.T = T; a.Nq = num_qo_heads; a.Nk = num_kv_heads; a.pos64 = positions_64;
-  a.eps = eps;
-  a.splits = head_splits(T, std::max(num_qo_heads, num_kv_heads));
+  a.positions = positions; a.T = T; a.pos64 = positions_64; a.eps = eps; a.partial = static_cast<float*>(workspace);
+  a.s[0].x = q; a.s[0].w = wq; a.s[0].g = gq; a.s[0].y = dq; a.s[0].stride = q_stride;
+  a.s[1].x = k; a.s[1].w = wk; a.s[1].g = gk; a.s[1].y = dk; a.s[1].stride = k_stride;
+  qk_bwd_streams(a, num_qo_heads, num_kv_heads);
   if (positions != nullptr) a.rot = rot_table(rope_theta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == SMLM_F16 ? launch_qk_bwd<__half>(a, dwq, dwk, st) : launch_qk_bwd<__nv_bfloat16>(a, dwq, dwk, st);

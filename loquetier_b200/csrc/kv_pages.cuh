@@ -37,15 +37,22 @@ __global__ void __launch_bounds__(kCpThreads) copy_pages_kernel(const CopyPagesA
     }
     const unsigned run = e * 16, gap = a.page_size * 16;   // chunks of a run, and from one run to the next
     const unsigned total = run * a.runs;
+    const unsigned hop = kCpThreads / max(run, 1u), rest = kCpThreads % max(run, 1u);   // runs and chunks of a thread's step
     for (unsigned c0 = blockIdx.x * kCpChunks + threadIdx.x; c0 < total; c0 += gridDim.x * kCpChunks) {
       uint4 v[kCpUnroll];
       unsigned at[kCpUnroll];
+      unsigned r = c0 / run, j = c0 % run;   // (one division per step of eight)
 #pragma unroll
       for (int u = 0; u < kCpUnroll; ++u) {
-        const unsigned ch = c0 + u * kCpThreads;
-        at[u] = run == gap ? ch : ch / max(run, 1u) * gap + ch % max(run, 1u);
+        at[u] = r * gap + j;
         v[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (ch < total) v[u] = __ldg(src + at[u]);
+        if (c0 + u * kCpThreads < total) v[u] = __ldg(src + at[u]);
+        r += hop;
+        j += rest;
+        if (j >= run) {
+          j -= run;
+          ++r;
+        }
       }
 #pragma unroll
       for (int u = 0; u < kCpUnroll; ++u)

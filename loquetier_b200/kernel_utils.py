@@ -173,33 +173,33 @@ class qk_norm_rope(Function):
     def forward(ctx: FunctionCtx, q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
                 k_weight: Optional[torch.Tensor], positions: Optional[torch.Tensor], base: float = 10000.0,
                 eps: float = 1e-6):
-        for t, name in ((q, "q"), (k, "k")):
-            ops.row_stride(t, name, ops.HEAD_DIM)
-        if k.size(0) != q.size(0) or q.size(1) == 0 or k.size(1) == 0:
+        strides = ops.row_stride(q, "q", ops.HEAD_DIM), ops.row_stride(k, "k", ops.HEAD_DIM)
+        rows, dtype, device = q.size(0), q.dtype, q.device
+        if k.size(0) != rows or q.size(1) == 0 or k.size(1) == 0:
             raise RuntimeError("q and k must have the same number of rows, and heads")
-        if (q_weight is None) != (k_weight is None):
-            raise RuntimeError("q_weight and k_weight must be given together")
-        if q_weight is None and positions is None:
-            raise RuntimeError("neither weights nor positions are given: nothing to do")
-        for t, name in ((k, "k"), (q_weight, "q_weight"), (k_weight, "k_weight")):
-            if t is not None and t.dtype != q.dtype:
-                raise RuntimeError(f"{name} must be {q.dtype} like q")
-        for t, name, n in ((q_weight, "q_weight", ops.HEAD_DIM), (k_weight, "k_weight", ops.HEAD_DIM),
-                           (positions, "positions", q.size(0))):
-            if t is not None:
+        if k.dtype != dtype or k.device != device:
+            raise RuntimeError(f"k must be {dtype} on {device} like q")
+        if q_weight is None or k_weight is None:
+            if q_weight is not k_weight:
+                raise RuntimeError("q_weight and k_weight must be given together")
+            if positions is None:
+                raise RuntimeError("neither weights nor positions are given: nothing to do")
+        else:
+            for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
                 ops._chk_cuda_contig(t, name, 1)
-                if t.numel() != n:
-                    raise RuntimeError(f"{name} must hold {n} values")
-        if positions is not None and positions.dtype not in (torch.int32, torch.int64):
-            raise RuntimeError("positions must be int32 or int64")
-        for t in (k, q_weight, k_weight, positions):
-            if t is not None and t.device != q.device:
-                raise RuntimeError(f"every tensor must be on {q.device}")
+                if t.numel() != ops.HEAD_DIM or t.dtype != dtype or t.device != device:
+                    raise RuntimeError(f"{name} must hold {ops.HEAD_DIM} values, {dtype} on {device} like q")
+        if positions is not None:
+            ops._chk_cuda_contig(positions, "positions", 1)
+            if positions.numel() != rows or positions.device != device:
+                raise RuntimeError(f"positions must hold {rows} values on {device}")
+            if positions.dtype not in (torch.int32, torch.int64):
+                raise RuntimeError("positions must be int32 or int64")
         ctx.save_for_backward(q, k, q_weight, k_weight, positions)
-        ctx.base, ctx.eps = base, eps
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        return ops.qk_norm_rope(yq, yk, q, k, q_weight, k_weight, positions, base, eps)
+        ctx.base, ctx.eps, ctx.strides = base, eps, strides
+        yq = torch.empty(q.shape, dtype=dtype, device=device)
+        yk = torch.empty(k.shape, dtype=dtype, device=device)
+        return ops.qk_norm_rope(yq, yk, q, k, q_weight, k_weight, positions, base, eps, strides)
 
     @staticmethod
     @once_differentiable
@@ -216,7 +216,7 @@ class qk_norm_rope(Function):
                 dwk.zero_()
         else:
             ops.qk_norm_rope_bwd(dq, dk, dwq, dwk, grad_q.contiguous(), grad_k.contiguous(), q, k, wq, wk, positions,
-                                 ctx.base, ctx.eps)
+                                 ctx.base, ctx.eps, ctx.strides)
         return dq, dk, dwq, dwk, None, None, None
 
 

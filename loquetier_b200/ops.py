@@ -434,28 +434,32 @@ def rms_norm_bwd(dx: torch.Tensor, dw: torch.Tensor, go: torch.Tensor, x: torch.
 HEAD_DIM = 128
 
 
-def qk_norm_rope(yq, yk, q, k, wq, wk, positions, base: float, eps: float):
-    """yq, yk = q, k normalised per head (weights given) and rotated (positions given); q and k may be strided rows."""
+def _row_strides(q, k):
+    return row_stride(q, "q", HEAD_DIM), row_stride(k, "k", HEAD_DIM)
+
+
+def qk_norm_rope(yq, yk, q, k, wq, wk, positions, base: float, eps: float, strides=None):
+    """yq, yk = q, k normalised per head (weights given) and rotated (positions given); q and k may be strided rows
+    (``strides``: their ``row_stride``, where it is known)."""
+    qs, ks = strides if strides is not None else _row_strides(q, k)
     with on_device(q):
         check(lib.smlm_b200_qk_norm_rope(yq.data_ptr(), yk.data_ptr(), q.data_ptr(), k.data_ptr(), _p(wq), _p(wk),
-                                         _p(positions), row_stride(q, "q", HEAD_DIM), row_stride(k, "k", HEAD_DIM),
-                                         int(q.size(0)), int(q.size(1)), int(k.size(1)), HEAD_DIM,
-                                         int(positions is not None and positions.dtype == torch.int64), float(base),
-                                         float(eps), _dtype_code(q), _stream(q)), "smlm_b200_qk_norm_rope")
+                                         _p(positions), qs, ks, q.size(0), q.size(1), k.size(1), HEAD_DIM,
+                                         int(positions is not None and positions.dtype == torch.int64), base, eps,
+                                         _dtype_code(q), _stream(q)), "smlm_b200_qk_norm_rope")
     return yq, yk
 
 
-def qk_norm_rope_bwd(dq, dk, dwq, dwk, gq, gk, q, k, wq, wk, positions, base: float, eps: float,
+def qk_norm_rope_bwd(dq, dk, dwq, dwk, gq, gk, q, k, wq, wk, positions, base: float, eps: float, strides=None,
                      workspace: Optional[torch.Tensor] = None):
     """Gradients of ``qk_norm_rope``; gq, gk, dq and dk contiguous, dwq and dwk in the storage type (None without weights)."""
-    T, Nq, Nk = int(q.size(0)), int(q.size(1)), int(k.size(1))
+    T, Nq, Nk = q.size(0), q.size(1), k.size(1)
+    qs, ks = strides if strides is not None else _row_strides(q, k)
     if workspace is None and wq is not None:
-        workspace = torch.empty(int(lib.smlm_b200_qk_norm_rope_bwd_workspace_bytes(T, Nq, Nk)), dtype=torch.uint8,
-                                device=q.device)
+        workspace = torch.empty(lib.smlm_b200_qk_norm_rope_bwd_workspace_bytes(T, Nq, Nk), dtype=torch.uint8, device=q.device)
     with on_device(q):
         check(lib.smlm_b200_qk_norm_rope_bwd(dq.data_ptr(), dk.data_ptr(), _p(dwq), _p(dwk), gq.data_ptr(), gk.data_ptr(),
                                              q.data_ptr(), k.data_ptr(), _p(wq), _p(wk), _p(positions), _p(workspace),
-                                             0 if workspace is None else workspace.numel(), row_stride(q, "q", HEAD_DIM),
-                                             row_stride(k, "k", HEAD_DIM), T, Nq, Nk, HEAD_DIM,
-                                             int(positions is not None and positions.dtype == torch.int64), float(base),
-                                             float(eps), _dtype_code(q), _stream(q)), "smlm_b200_qk_norm_rope_bwd")
+                                             0 if workspace is None else workspace.numel(), qs, ks, T, Nq, Nk, HEAD_DIM,
+                                             int(positions is not None and positions.dtype == torch.int64), base, eps,
+                                             _dtype_code(q), _stream(q)), "smlm_b200_qk_norm_rope_bwd")
