@@ -60,7 +60,7 @@ constexpr int kPfKvBytes = 2 * kPfKeys * 128;     // two 64-dim panels of [keys]
 constexpr int kPfKOff = kPfQBytes;
 constexpr int kPfVOff = kPfKOff + kPfStages * kPfKvBytes;
 constexpr int kPfBarOff = kPfVOff + kPfStages * kPfKvBytes;
-constexpr int kPfSmem = kPfBarOff + 4 * kPfStages * 8 + 80;   // the rings' barriers, 8 more, the tensor-memory address
+constexpr int kPfSmem = kPfBarOff + 4 * kPfStages * 8 + 88;   // the rings' barriers, 9 more, the tensor-memory address
 constexpr int kPfOCol = kPfSBufs * kPfKeys;       // first column of O
 constexpr int kPfTmemCols = 256;                  // S buffers + O (128 columns)
 constexpr int kPfCtasPerSm = 2;
@@ -340,9 +340,11 @@ __global__ void __launch_bounds__(kPfThreads, kPfCtasPerSm) paged_prefill_kernel
   // o_done: two barriers used by alternate tiles.  A softmax thread consumes the completion of tile j - 1
   // after it has released tile j; with a single barrier the product of tile j could complete in between and
   // the parity of tile j - 1 could no longer be told from that of tile j + 1.
-  const uint32_t p_full = s_full + 32, o_done = s_full + 40, q_full = s_full + 56;
-  const uint32_t tmem_slot = s_full + 64;
-  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(pf_smem + kPfBarOff + 4 * NS * 8 + 64);
+  // p_full likewise: a softmax warp may hand on tile j + 1 before a slower one - one that rescales its rows - has handed on
+  // tile j, and on a single barrier the two arrivals would count for the same tile.
+  const uint32_t p_full = s_full + 32, o_done = s_full + 48, q_full = s_full + 64;
+  const uint32_t tmem_slot = s_full + 72;
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(pf_smem + kPfBarOff + 4 * NS * 8 + 72);
 
   T* O = static_cast<T*>(a.o);
   if (ntiles == 0) {   // no key is visible: zeros
@@ -387,6 +389,7 @@ __global__ void __launch_bounds__(kPfThreads, kPfCtasPerSm) paged_prefill_kernel
       mbar_init(s_empty + i * 8, 1);   // P lives in the S buffer: freed by the commit of P . V
     }
     mbar_init(p_full, 2 * kPfRows);
+    mbar_init(p_full + 8, 2 * kPfRows);
     mbar_init(o_done, 1);
     mbar_init(o_done + 8, 1);
     mbar_init(q_full, 2 * kPfRows);
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(kPfThreads, kPfCtasPerSm) paged_prefill_kernel
         const int st = j % NS;
         pf_wait_role(v_full + st * 8, (j / NS) & 1, a.err, dead);
         PF_STAMP(1, j, 1);
-        pf_wait_role(p_full, j & 1, a.err, dead);
+        pf_wait_role(p_full + (j & 1) * 8, (j >> 1) & 1, a.err, dead);
         PF_STAMP(1, j, 2);
         tc_fence_after();
         if (!dead) {
@@ -660,7 +663,7 @@ __global__ void __launch_bounds__(kPfThreads, kPfCtasPerSm) paged_prefill_kernel
       tc_wait_st();
       if (tid == 0) PF_STAMP(0, j, 6);
       tc_fence_before();
-      mbar_arrive(p_full);
+      mbar_arrive(p_full + (j & 1) * 8);
       wait_prev();   // every phase of the barrier is consumed, so that its parity stays readable
       if (tid == 0) PF_STAMP(0, j, 7);
     }
