@@ -35,7 +35,9 @@ struct ExPlan {
   int qt;          // quarters of 32 rows of a row tile
   int shares;      // CTAs per kv head
   int min_tiles;   // key tiles of a share at least
-  size_t bytes;    // of softmax states
+  bool dense;      // the keys are rotated once, in front
+  size_t state;    // bytes of cuts and softmax states
+  size_t bytes;    // and of rotated keys
 };
 
 ExPlan extend_plan(int batch, int total_q, int total_pages, int page_size, int num_kv_heads, int group) {
@@ -49,14 +51,21 @@ ExPlan extend_plan(int batch, int total_q, int total_pages, int page_size, int n
   const long long key_tiles = static_cast<long long>(total_pages) * page_size / kXtKeys + batch;
   const long long most = (all_rows / rows + batch) * key_tiles / p.min_tiles + 1;
   p.shares = static_cast<int>(std::min<long long>(std::max(1, kXtCtasPerSm * kNumSMs / num_kv_heads), most));
-  p.bytes = p.shares > 1 ? static_cast<size_t>(p.shares) * num_kv_heads * (sizeof(ExCut) + 2 * rows * kPdRec * sizeof(float)) : 0;
+  p.state = p.shares > 1 ? static_cast<size_t>(p.shares) * num_kv_heads * (sizeof(ExCut) + 2 * rows * kPdRec * sizeof(float)) : 0;
+  p.dense = p.qt == 4 && mean >= 256;
+  p.bytes = p.state + (p.dense ? static_cast<size_t>(total_pages) * page_size * num_kv_heads * kPdDim * 2 : 0);
   return p;
 }
 
-template <typename T, int QT>
+template <typename T, int QT, bool DENSE = false>
 int launch_extend(const ExArgs& a, const ExPlan& p, cudaStream_t stream) {
+  using X = Xt<QT, DENSE>;
   const unsigned heads = static_cast<unsigned>(a.num_kv_heads);
-  const int rc = launch(paged_extend_kernel<T, QT>, dim3(p.shares * heads, 1, 1), Xt<QT>::kThreads, 1, Xt<QT>::kSmem, stream, a);
+  if (DENSE) {
+    const int rc = launch(extend_rotate_kernel<T>, dim3(a.total_pages, 1, 1), 128, 1, 0, stream, a);
+    if (rc != SMLM_OK) return rc;
+  }
+  const int rc = launch(paged_extend_kernel<T, QT, DENSE>, dim3(p.shares * heads, 1, 1), X::kThreads, 1, X::kSmem, stream, a);
   if (rc != SMLM_OK || p.shares == 1) return rc;
   return launch(paged_extend_merge_kernel<T, QT>, dim3((p.shares - 1) * heads, kXtMergeSplit, 1), kXtMergeThreads, 1, 0, stream, a);
 }
@@ -66,7 +75,7 @@ int dispatch_extend(const ExArgs& a, const ExPlan& p, cudaStream_t stream) {
   switch (p.qt) {
     case 1: return launch_extend<T, 1>(a, p, stream);
     case 2: return launch_extend<T, 2>(a, p, stream);
-    default: return launch_extend<T, 4>(a, p, stream);
+    default: return p.dense ? launch_extend<T, 4, true>(a, p, stream) : launch_extend<T, 4>(a, p, stream);
   }
 }
 
@@ -175,7 +184,8 @@ int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, con
   ExArgs a;
   a.o = o; a.q = q; a.qo_indptr = qo_indptr; a.kv_ptrs = kv_ptrs; a.kv_indptr = kv_indptr;
   a.last_page_offset = last_page_offset; a.err = status_word;
-  a.cuts = p.bytes > 0 ? static_cast<ExCut*>(workspace) : nullptr;
+  a.cuts = p.state > 0 ? static_cast<ExCut*>(workspace) : nullptr;
+  a.dense = p.dense ? static_cast<char*>(workspace) + p.state : nullptr;
   a.partial = reinterpret_cast<float*>(a.cuts + static_cast<size_t>(p.shares) * num_kv_heads);
   a.batch = batch_size; a.total_q = total_q; a.total_pages = total_pages; a.num_kv_heads = num_kv_heads;
   a.num_layers = num_layers; a.layer_idx = layer_idx; a.page_size = page_size;

@@ -28,6 +28,7 @@
 // Every wait is bounded.
 #pragma once
 #include "paged_prefill.cuh"
+#include "rms_norm.cuh"
 #include "rotary.cuh"
 
 namespace smlm {
@@ -52,6 +53,7 @@ struct ExArgs {
   const int32_t* last_page_offset;  // [B]
   float* partial;                 // states [shares][2][Nkv][rows of a tile][kPdRec]: a share cuts two row tiles at most
   ExCut* cuts;                    // [shares][Nkv]
+  void* dense;                    // rotated keys [Nkv][total_pages * page_size][128], or null
   int* err;                       // error word, may be null
   int batch, total_q, total_pages, num_kv_heads, num_layers, layer_idx, page_size;
   int lg;                         // log2 of the query heads per kv head, G
@@ -239,12 +241,12 @@ __device__ __forceinline__ void ex_layout(const ExArgs& a, long long w0, long lo
   __syncthreads();
 }
 
-template <int QT>
+template <int QT, bool DENSE = false>
 struct Xt {
   static constexpr int kRows = 32 * QT;
   static constexpr int kStages = QT == 4 ? 2 : 3;       // of the K ring and of the V ring
   static constexpr int kSegs = QT == 2 ? 4 : 16;
-  static constexpr int kRotWarps = 4;
+  static constexpr int kRotWarps = DENSE ? 0 : 4;
   static constexpr int kThreads = 32 * (2 * QT + kRotWarps + 4);
   static constexpr int kQPanel = kRows * 128;           // Q: two 64-dim panels of [rows][128 B]
   static constexpr int kKOff = 2 * kQPanel;
@@ -283,9 +285,9 @@ __device__ __forceinline__ uint64_t load_if(const void* const* at, bool yes) {
 }
 
 // grid: shares * Nkv
-template <typename T, int QT>
-__global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_kernel(const __grid_constant__ ExArgs a) {
-  using X = Xt<QT>;
+template <typename T, int QT, bool DENSE>
+__global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_extend_kernel(const __grid_constant__ ExArgs a) {
+  using X = Xt<QT, DENSE>;
   constexpr int ROWS = X::kRows, NS = X::kStages, ROTATORS = 32 * X::kRotWarps;
   extern __shared__ __align__(1024) unsigned char xt_smem[];
   const int tid = threadIdx.x, lane = tid & 31;
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_k
   // (cos, cos, sin, sin) of the turn from one of a loader's keys to the next, two frequencies each
   float* turn = reinterpret_cast<float*>(xt_smem + X::kTurnOff);
   ExScratch<X::kSegs>& sc = *reinterpret_cast<ExScratch<X::kSegs>*>(xt_smem + X::kScratchOff);
-  if (tid < 64) {
+  if (!DENSE && tid < 64) {
     float sn, cs;
     rot_sincos(static_cast<float>(ROTATORS / 8), a.rot.hi[tid], a.rot.lo[tid], &sn, &cs);
     turn[(tid >> 1) * 4 + (tid & 1)] = cs;
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_k
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(k_raw + i * 8, 32);
-      mbar_init(k_full + i * 8, ROTATORS);
+      mbar_init(k_full + i * 8, DENSE ? 32 : ROTATORS);
       mbar_init(k_empty + i * 8, 1);
       mbar_init(v_full + i * 8, 32);
       mbar_init(v_empty + i * 8, 1);
@@ -362,9 +364,9 @@ __global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_k
 
   for (;;) {
     const int count = sc.count;
-    if (role == 0) {
+    if (!DENSE && role == 0) {
       // ---------------- rotators: thread = (chunk c of 8 dims and its partner, every STEP-th key) ----------------
-      constexpr int STEP = ROTATORS / 8, KPT = kXtKeys / STEP;   // keys of a thread per tile
+      constexpr int STEP = DENSE ? 32 : ROTATORS / 8, KPT = kXtKeys / STEP;   // keys of a thread per tile
       const int rt = other * 32 + lane, c = rt & 7, kr = rt >> 3;
       const ulonglong2* my_turn = reinterpret_cast<const ulonglong2*>(turn) + c * 4;
       uint64_t cc[4] = {}, ss[4] = {};   // cosines and sines of key kr + STEP i, two frequencies each
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_k
       }
     } else if (role == 1 || role == 2) {
       // ---------------- loaders: a warp copies a tile, a lane chunk lane & 15 of the keys 2 i + (lane >> 4) ----------------
-      const uint32_t ring = role == 1 ? ks0 : vs0, full = role == 1 ? k_raw : v_full, empty = role == 1 ? k_empty : v_empty;
+      const uint32_t ring = role == 1 ? ks0 : vs0, full = role == 2 ? v_full : DENSE ? k_full : k_raw, empty = role == 1 ? k_empty : v_empty;
       const int lp = 31 - __clz(P);   // the page size is a power of two (checked by the host)
       const uint32_t head_off =
           static_cast<uint32_t>(((a.layer_idx * 2 + role - 1) * a.num_kv_heads + kvh) * P) * 256u;   // bytes
@@ -439,8 +441,12 @@ __global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_k
       bool bad_ptr = false;
       // eight keys lie in one page: lane e looks after the keys 8 e .. 8 e + 7 of the tile, a tile ahead of the copies
       const int e8 = (lane & 7) * 8;
-      auto entry = [&](const ExSeg& s, int tile) {
+      const bool rows = DENSE && role == 1;   // rotated keys lie one after the other, the pages' places for them in order
+      auto entry = [&](const ExSeg& s, int tile) -> uint64_t {
         const int key = tile * kXtKeys + e8;
+        if (rows)
+          return key < s.nkeys ? reinterpret_cast<uint64_t>(a.dense) +
+                                     ((static_cast<uint64_t>(kvh) * a.total_pages + s.p0) * P + key) * 256u : 0;
         return load_if(a.kv_ptrs + s.p0 + (key >> lp), key < s.nkeys);
       };
       int seg = 0;
@@ -454,7 +460,7 @@ __global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_k
           const int key0 = (tile0 + j) * kXtKeys;
           const bool ok = page != 0 && (page & 15) == 0;
           bad_ptr |= key0 + e8 < nkeys && !ok;
-          const uint64_t base = page + head_off + ((key0 + e8) & (P - 1)) * 256u;
+          const uint64_t base = rows ? page : page + head_off + ((key0 + e8) & (P - 1)) * 256u;
           const bool whole = __all_sync(0xffffffffu, ok) && key0 + kXtKeys <= nkeys;
           const uint64_t mine = ok ? base : 0;
           page = j + 1 < ntiles ? entry(sc.seg[seg], tile0 + j + 1) : next < count ? entry(sc.seg[next], sc.seg[next].tile0) : 0;
@@ -502,6 +508,7 @@ __global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_k
           for (int j = 0; j < ntiles; ++j, ++g) {
             const int st = g % NS, sb = g & 1;
             pf_wait_role(k_full + st * 8, (g / NS) & 1, a.err, dead);
+            if (DENSE) fence_proxy_async();   // K came by the loader's ordinary copies
             if (g >= 2) pf_wait_role(o_done + sb * 8, ((g >> 1) - 1) & 1, a.err, dead);   // P . V has read this S buffer
             tc_fence_after();
             if (!dead) {
@@ -748,6 +755,57 @@ __global__ void __launch_bounds__(Xt<QT>::kThreads, kXtCtasPerSm) paged_extend_k
   __syncthreads();
   tc_fence_after();
   if (role == 3) tc_dealloc(tmem, kXtTmemCols);
+}
+
+// The keys of all pages rotated, for chunks of several row tiles, which would each rotate them again: one CTA per page, a
+// thread (entry, chunk of 8 dims and its partner), whose sines serve all kv heads.
+template <typename T>
+__global__ void __launch_bounds__(128) extend_rotate_kernel(const __grid_constant__ ExArgs a) {
+  __shared__ __align__(16) float freq[128];
+  load_rot_table(a.rot, freq);
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  const int pg = blockIdx.x, P = a.page_size;
+  int lo = 0, hi = a.batch;   // the request of the page: the last one that starts at or before it
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.kv_indptr[mid] <= pg) lo = mid; else hi = mid;
+  }
+  const ExRequest r = ex_request(a, lo);
+  const int first = (pg - r.p0) * P;   // position of the page's first entry
+  if (r.n == 0 || first < 0 || first >= r.len) return;
+  const T* page = static_cast<const T*>(a.kv_ptrs[pg]);
+  if (page == nullptr || (reinterpret_cast<uintptr_t>(page) & 15) != 0) page = nullptr;   // (reported by the loader of V)
+  T* out = static_cast<T*>(a.dense) + static_cast<size_t>(pg) * P * kPdDim;
+  const size_t head_step = static_cast<size_t>(a.total_pages) * P * kPdDim;
+  for (int i = threadIdx.x; i < P * 8; i += 128) {
+    const int e = i >> 3, c = i & 7;
+    if (first + e >= r.len) break;
+    float cs[8], sn[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      rot_sincos(static_cast<float>(first + e), freq[c * 8 + k], freq[64 + c * 8 + k], &sn[k], &cs[k]);
+    const T* src = page + (static_cast<size_t>(a.layer_idx) * 2 * a.num_kv_heads * P + e) * kPdDim + c * 8;
+    T* dst = out + static_cast<size_t>(e) * kPdDim + c * 8;
+    for (int h = 0; h < a.num_kv_heads; ++h, src += P * kPdDim, dst += head_step) {
+      float x[8], y[8], u[8], v[8];
+      uint4 xo = make_uint4(0u, 0u, 0u, 0u), yo = xo;
+      if (page != nullptr) {
+        xo = __ldcs(reinterpret_cast<const uint4*>(src));
+        yo = __ldcs(reinterpret_cast<const uint4*>(src + 64));
+      }
+      unpack8<T>(xo, x);
+      unpack8<T>(yo, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        u[k] = x[k] * cs[k] - y[k] * sn[k];
+        v[k] = y[k] * cs[k] + x[k] * sn[k];
+      }
+      *reinterpret_cast<uint4*>(dst) = pack8<T>(u);
+      *reinterpret_cast<uint4*>(dst + 64) = pack8<T>(v);
+    }
+  }
 }
 
 // Merges the states of the row tiles that are cut, in the order of the keys.  grid: ((shares - 1) * Nkv, kXtMergeSplit); a
