@@ -36,6 +36,7 @@ struct ExPlan {
   int shares;      // CTAs per kv head
   int min_tiles;   // key tiles of a share at least
   bool dense;      // the keys are rotated once, in front
+  bool fits;       // the work counts in 31 bits
   size_t state;    // bytes of cuts and softmax states
   size_t bytes;    // and of rotated keys
 };
@@ -50,6 +51,7 @@ ExPlan extend_plan(int batch, int total_q, int total_pages, int page_size, int n
   // all the CTAs that are resident, but no more than the work can hold
   const long long key_tiles = static_cast<long long>(total_pages) * page_size / kXtKeys + batch;
   const long long most = (all_rows / rows + batch) * key_tiles / p.min_tiles + 1;
+  p.fits = (all_rows / rows + batch) * key_tiles < 0x7fffff00LL;
   p.shares = static_cast<int>(std::min<long long>(std::max(1, kXtCtasPerSm * kNumSMs / num_kv_heads), most));
   p.state = p.shares > 1 ? static_cast<size_t>(p.shares) * num_kv_heads * (sizeof(ExCut) + 2 * rows * kPdRec * sizeof(float)) : 0;
   p.dense = p.qt == 4 && mean >= 256;
@@ -177,6 +179,7 @@ int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, con
       static_cast<long long>(num_layers) * 2 * num_kv_heads * page_size * kPdDim * 2 > 0x7fffffffLL)   // a page of 2 GB
     return SMLM_ERR_INVALID_ARGUMENT;
   const ExPlan p = extend_plan(batch_size, total_q, total_pages, page_size, num_kv_heads, group);
+  if (!p.fits) return SMLM_ERR_INVALID_ARGUMENT;
   if (p.bytes > 0) {
     if (workspace == nullptr || workspace_bytes < p.bytes) return SMLM_ERR_WORKSPACE;
     if (!aligned16(workspace)) return SMLM_ERR_MISALIGNED;

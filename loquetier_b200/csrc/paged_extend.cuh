@@ -93,53 +93,52 @@ template <int ROWS>
 __device__ __forceinline__ int ex_row_tiles(const ExArgs& a, const ExRequest& r) {
   return ((r.n << a.lg) + ROWS - 1) / ROWS;
 }
-// key tiles of each of a request's row tiles (one at least: rows that see no key still have to be written)
-__device__ __forceinline__ int ex_key_tiles(const ExRequest& r) { return max(1, (r.len + kXtKeys - 1) / kXtKeys); }
+// Key tiles of a request's row tiles in front of row tile x, together: the keys that the last row of each sees, in tiles of
+// 64.  Row tile t ends with query (t + 1) q - 1, q the queries of a row tile, and sees pos0 + (t + 1) q keys, the last one
+// all; q is a power of two, so the sum has a closed form.  A request with more queries than keys (an error) counts one key
+// tile for every row tile of it more than it can see, as all of its row tiles have to be written.
+template <int ROWS>
+__device__ __forceinline__ int ex_before(const ExArgs& a, const ExRequest& r, int x) {
+  const int all = ex_row_tiles<ROWS>(a, r);
+  const int most = max(1, (r.len + kXtKeys - 1) / kXtKeys);
+  if (r.len < r.n) return x * most;
+  const int y = min(x, all - 1);                      // of these the closed form holds
+  const int lq = 31 - __clz(ROWS) - a.lg;             // log2 of q
+  const int first = r.len - r.n + (1 << lq) + kXtKeys - 1;   // row tile t: (first + t q) / 64, rounded down
+  int sum;
+  if (lq >= 6) {
+    sum = y * (first >> 6) + ((y * (y - 1)) >> 1 << (lq - 6));
+  } else {                                            // the quotients go up by one every m = 64 / q row tiles
+    const int lm = 6 - lq, f = first >> lq;
+    auto steps = [&](unsigned i) {                    // sum of j >> lm for j < i, modulo 2^32: the difference is what counts
+      const unsigned t = i >> lm;
+      return (((t & 1) ? t * ((t - 1) >> 1) : (t >> 1) * (t - 1)) << lm) + t * (i - (t << lm));
+    };
+    sum = static_cast<int>(steps(f + y) - steps(f));
+  }
+  return x == all ? sum + most : sum;
+}
+template <int ROWS>
+__device__ __forceinline__ int ex_work(const ExArgs& a, const ExRequest& r) {
+  return r.n > 0 ? ex_before<ROWS>(a, r, ex_row_tiles<ROWS>(a, r)) : 0;
+}
 
 // A run of key tiles of one row tile.
 struct ExSeg {
   int qo0, row0, nrows;   // first row of q of the request; of its rows, the tile's first and their number
   int pos0, p0;           // position of the request's first new token; first page in the table
   int nkeys;              // keys that a row of the tile sees
-  int tile0, ntiles;      // the run, cut where no row sees a key any more (one tile at least of a row tile's first run)
+  int tile0, ntiles;      // the run
   int part;               // where its state goes: 0, 1, or negative: the row tile is finished here
 };
 
 template <int SEGS>
 struct ExScratch {
   long long sum[16];
-  long long begin, end, next;   // of the share's work; where the next round of runs starts
+  int begin, end, next;         // of the share's work; where the next round of runs starts
   int count;
   ExSeg seg[SEGS];              // runs of the share that are laid out at a time
 };
-
-// the sum over the CTA's NT threads
-template <int NT, typename S>
-__device__ __forceinline__ long long ex_sum(long long v, S& sc) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sc.sum[threadIdx.x >> 5] = v;
-  __syncthreads();
-  long long t = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 32; ++w) t += sc.sum[w];
-  return t;
-}
-
-// Key tiles of a share.  Every thread of the CTA takes part; `report`: what is wrong with the index arrays is written down.
-template <int ROWS, int NT, typename S>
-__device__ __forceinline__ long long ex_share(const ExArgs& a, bool report, S& sc) {
-  long long work = 0;
-  for (int b = threadIdx.x; b < a.batch; b += NT) {
-    const ExRequest r = ex_request(a, b);
-    if (report && r.bad != 0 && a.err != nullptr) atomicOr(a.err, r.bad);
-    work += static_cast<long long>(ex_row_tiles<ROWS>(a, r)) * ex_key_tiles(r);
-  }
-  work = ex_sum<NT>(work, sc);
-  const long long even = (work + a.shares - 1) / a.shares;
-  return even > a.min_tiles ? even : a.min_tiles;
-}
 
 // Running sums over the CTA's threads in their order: returns what the threads before this one hold, `all` the whole.
 template <int NT, typename S>
@@ -167,10 +166,9 @@ __device__ __forceinline__ long long ex_scan(long long v, long long& all, S& sc)
 // What the merge of the row tile that a share starts inside of needs to know.
 struct ExCut {
   int qo0, row0, nrows;   // as in ExSeg; no rows: the share starts a row tile, or holds no work
-  int first, count;       // the row tile's first share, and the number of its shares whose rows see a key
-  int shares;             // all of its shares but the first: that many CTAs merge
+  int first, shares;      // the row tile's first share, and how many more it lies in: that many CTAs merge
   int part;               // where the first share has its state; the others have it at 0
-  int pad;
+  int pad[2];
 };
 
 // keys that a row of row tile `tile` of the request sees
@@ -180,60 +178,102 @@ __device__ __forceinline__ int ex_visible(const ExArgs& a, const ExRequest& r, i
   return max(0, min(r.len, r.len - r.n + (last >> a.lg) + 1));
 }
 
-// Lays out the share's runs from `w0` on, in order, as many as fit.  The first round also writes down the cut that the
-// share starts with (cut: its place, null for other rounds).
+// A thread's request of those that the CTA looks at together, its work and its place in the head's work.
+struct ExMine {
+  ExRequest r;
+  int work, at;
+};
+
+// Requests b0 + thread; `before`: the work in front of them, and behind them on return
+template <int ROWS, int NT, typename S>
+__device__ __forceinline__ ExMine ex_mine(const ExArgs& a, int b0, long long& before, S& sc) {
+  const int b = b0 + threadIdx.x;
+  ExMine m = {};
+  if (b < a.batch) {
+    m.r = ex_request(a, b);
+    m.work = ex_work<ROWS>(a, m.r);
+  }
+  long long all;
+  const long long at = before + ex_scan<NT>(m.work, all, sc);
+  before += all;
+  m.at = static_cast<int>(min(at, 0x7fffffffLL));   // (more work than that is refused, see ex_share)
+  return m;
+}
+
+// Key tiles of a share, 0 where the index arrays make no sense together.  m: the first NT requests.  `report`: what is wrong
+// with the index arrays is written down.
+template <int ROWS, int NT, typename S>
+__device__ __forceinline__ int ex_share(const ExArgs& a, bool report, ExMine& m, S& sc) {
+  long long work = 0;
+  int bad = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += NT) {
+    const ExMine next = ex_mine<ROWS, NT>(a, b0, work, sc);
+    bad |= next.r.bad;
+    if (b0 == 0) m = next;
+  }
+  if (work > 0x7fffffffLL - kXtKeys) bad |= kErrBadIndptr;   // sound arrays stay below: the host has checked their sizes
+  if (report && bad != 0 && a.err != nullptr) atomicOr(a.err, bad);
+  if (work > 0x7fffffffLL - kXtKeys) return 0;
+  const unsigned w = static_cast<unsigned>(work);
+  return max(static_cast<int>((w + a.shares - 1) / a.shares), a.min_tiles);
+}
+
+// Lays out the share's runs from `w0` on, in order, as many as fit.  m: the first NT requests.  The first round also writes
+// down the cut that the share starts with (cut: its place, null for other rounds).
 template <int ROWS, int NT, int SEGS>
-__device__ __forceinline__ void ex_layout(const ExArgs& a, long long w0, long long per, ExCut* cut, ExScratch<SEGS>& sc) {
-  const long long w_begin = sc.begin, w_end = sc.end;
+__device__ __forceinline__ void ex_layout(const ExArgs& a, int w0, unsigned per, const ExMine& m0, ExCut* cut,
+                                          ExScratch<SEGS>& sc) {
+  const int w_begin = sc.begin, w_end = sc.end;
   if (threadIdx.x == 0) sc.next = w_end;
   long long before = 0, segs = 0;
   bool wrote = false;
   for (int b0 = 0; b0 < a.batch && before < w_end && segs < SEGS; b0 += NT) {
-    const int b = b0 + threadIdx.x;
-    ExRequest r = {};
-    long long mine = 0;
-    int nt = 1;
-    if (b < a.batch) {
-      r = ex_request(a, b);
-      nt = ex_key_tiles(r);
-      mine = static_cast<long long>(ex_row_tiles<ROWS>(a, r)) * nt;
+    const ExMine m = a.batch <= NT ? m0 : ex_mine<ROWS, NT>(a, b0, before, sc);
+    const int from = max(w0, m.at) - m.at, to = min(w_end - m.at, m.work);   // of the request's work
+    int first = 0, n = 0;   // its row tiles in the share
+    if (from < to) {
+      const int all = ex_row_tiles<ROWS>(a, m.r);
+      auto tile_at = [&](int w) {   // the row tile that holds w
+        int lo = 0, hi = all;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (ex_before<ROWS>(a, m.r, mid) <= w) lo = mid; else hi = mid;
+        }
+        return lo;
+      };
+      first = tile_at(from);
+      n = tile_at(to - 1) - first + 1;
     }
-    long long all, all_segs;
-    const long long at = before + ex_scan<NT>(mine, all, sc);
-    const long long from = max(w0, at), to = min(w_end, at + mine);
-    const int first = from < to ? static_cast<int>((from - at) / nt) : 0;          // row tiles in the share
-    const int n = from < to ? static_cast<int>((to - 1 - at) / nt) - first + 1 : 0;
-    long long i = segs + ex_scan<NT>(n, all_segs, sc);
+    long long all_segs;
+    int i = static_cast<int>(min(segs + ex_scan<NT>(n, all_segs, sc), static_cast<long long>(SEGS)));
     for (int tile = first; tile < first + n && i < SEGS; ++tile, ++i) {
-      const long long start = at + static_cast<long long>(tile) * nt;
-      const int k0 = static_cast<int>(max(from, start) - start), k1 = static_cast<int>(min(to, start + nt) - start);
+      const int start = ex_before<ROWS>(a, m.r, tile), nt = ex_before<ROWS>(a, m.r, tile + 1) - start;
+      const int k0 = max(from, start) - start, k1 = min(to, start + nt) - start;
       ExSeg s;
-      s.qo0 = r.qo0;
+      s.qo0 = m.r.qo0;
       s.row0 = tile * ROWS;
-      s.nrows = min(ROWS, (r.n << a.lg) - s.row0);
-      s.pos0 = r.len - r.n;
-      s.p0 = r.p0;
-      s.nkeys = ex_visible<ROWS>(a, r, tile);
-      const int seen = max(1, (s.nkeys + kXtKeys - 1) / kXtKeys);
+      s.nrows = min(ROWS, (m.r.n << a.lg) - s.row0);
+      s.pos0 = m.r.len - m.r.n;
+      s.p0 = m.r.p0;
+      s.nkeys = ex_visible<ROWS>(a, m.r, tile);
       s.tile0 = k0;
-      s.ntiles = max(0, min(k1, seen) - k0);
-      s.part = k0 == 0 && k1 == nt ? -1 : start + k0 == w_begin ? 0 : 1;
+      s.ntiles = k1 - k0;
+      s.part = k0 == 0 && k1 == nt ? -1 : m.at + start + k0 == w_begin ? 0 : 1;
       sc.seg[i] = s;
-      if (i == SEGS - 1) sc.next = start + k1;
+      if (i == SEGS - 1) sc.next = m.at + start + k1;
       if (cut != nullptr && i == 0 && k0 > 0) {
+        const unsigned begin = m.at + start;
         ExCut c;
         c.qo0 = s.qo0; c.row0 = s.row0; c.nrows = s.nrows;
-        c.first = static_cast<int>(start / per);
-        c.shares = static_cast<int>((start + nt - 1) / per) - c.first;
-        c.count = static_cast<int>((start + seen - 1) / per) - c.first + 1;
-        c.part = start == c.first * per ? 0 : 1;
-        c.pad = 0;
+        c.first = begin / per;
+        c.shares = (begin + nt - 1) / per - c.first;
+        c.part = begin == c.first * per ? 0 : 1;
+        c.pad[0] = c.pad[1] = 0;
         *cut = c;
         wrote = true;
       }
     }
     segs += all_segs;
-    before += all;
   }
   if (cut != nullptr && !__syncthreads_or(wrote) && threadIdx.x == 0) cut->nrows = 0;
   __syncthreads();
@@ -310,10 +350,12 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
     return;
   }
   const int kvh = blockIdx.x % a.num_kv_heads, share = blockIdx.x / a.num_kv_heads;
-  const long long per = ex_share<ROWS, X::kThreads>(a, blockIdx.x == 0, sc);
+  ExMine mine;
+  const int per = ex_share<ROWS, X::kThreads>(a, blockIdx.x == 0, mine, sc);
   if (tid == 0) {
-    sc.begin = share * per;
-    sc.end = sc.begin + per;
+    const long long begin = static_cast<long long>(share) * per;
+    sc.begin = static_cast<int>(min(begin, 0x7fffffffLL));
+    sc.end = static_cast<int>(min(begin + per, 0x7fffffffLL));
   }
   __syncthreads();
   const int gmask = (1 << a.lg) - 1;
@@ -332,7 +374,7 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
   const int other = warp - (warp < 4 ? min(warp, QT) : warp < 8 ? QT + min(warp - 4, QT) : 2 * QT);
   const int role = softmax ? -1 : max(0, other - X::kRotWarps + 1);   // 0 rotator, 1 K, 2 V, 3 S, 4 O
 
-  ex_layout<ROWS, X::kThreads>(a, sc.begin, per, a.cuts == nullptr ? nullptr : a.cuts + blockIdx.x, sc);
+  ex_layout<ROWS, X::kThreads>(a, sc.begin, per, mine, a.cuts == nullptr ? nullptr : a.cuts + blockIdx.x, sc);
   if (sc.count == 0) return;   // nothing left for this share (uniform over the CTA)
 
   if (tid == 0) {
@@ -449,13 +491,10 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
                                      ((static_cast<uint64_t>(kvh) * a.total_pages + s.p0) * P + key) * 256u : 0;
         return load_if(a.kv_ptrs + s.p0 + (key >> lp), key < s.nkeys);
       };
-      int seg = 0;
-      while (seg < count && sc.seg[seg].ntiles == 0) ++seg;
-      uint64_t page = seg < count ? entry(sc.seg[seg], sc.seg[seg].tile0) : 0;
-      while (seg < count) {
+      uint64_t page = entry(sc.seg[0], sc.seg[0].tile0);
+      for (int seg = 0; seg < count && !dead; ++seg) {
         const int tile0 = sc.seg[seg].tile0, ntiles = sc.seg[seg].ntiles, nkeys = sc.seg[seg].nkeys;
-        int next = seg + 1;
-        while (next < count && sc.seg[next].ntiles == 0) ++next;
+        const int next = seg + 1;
         for (int j = 0; j < ntiles; ++j, ++g) {
           const int key0 = (tile0 + j) * kXtKeys;
           const bool ok = page != 0 && (page & 15) == 0;
@@ -491,8 +530,6 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
           }
           cp_async_arrive(full + st * 8);   // when this lane's copies have landed
         }
-        if (dead) break;
-        seg = next;
       }
       cp_async_wait<0>();
       if (__any_sync(0xffffffffu, bad_ptr) && lane == 0 && a.err != nullptr) atomicOr(a.err, kErrBadPointer);
@@ -503,7 +540,6 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
         const uint64_t qdesc = desc_kmajor(qs), kdesc = desc_kmajor(ks0);   // (addresses are added below: no field overflows)
         for (int seg = 0; seg < count; ++seg) {
           const int ntiles = sc.seg[seg].ntiles;
-          if (ntiles == 0) continue;
           pf_wait_role(q_full, gs & 1, a.err, dead);
           for (int j = 0; j < ntiles; ++j, ++g) {
             const int st = g % NS, sb = g & 1;
@@ -562,7 +598,6 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
       const uint32_t o_tmem = my_tmem + kXtOCol + half * 64;
       for (int seg = 0; seg < count; ++seg) {
         const ExSeg s = sc.seg[seg];
-        if (s.ntiles == 0) continue;
         const int rr = s.row0 + row;
         // rows past the end behave like the last one
         const int my_pos = s.pos0 + (min(rr, s.row0 + s.nrows - 1) >> a.lg);
@@ -744,9 +779,11 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
       }
     }
     if (sc.next >= sc.end) break;
-    const long long w0 = sc.next;
+    const int w0 = sc.next;
     __syncthreads();   // everyone is done with this round's runs
-    ex_layout<ROWS, X::kThreads>(a, w0, 1, nullptr, sc);
+    long long before = 0;
+    if (a.batch <= X::kThreads) mine = ex_mine<ROWS, X::kThreads>(a, 0, before, sc);
+    ex_layout<ROWS, X::kThreads>(a, w0, 1u, mine, nullptr, sc);
     if (sc.count == 0) break;
   }
 
@@ -823,7 +860,7 @@ __global__ void __launch_bounds__(kXtMergeThreads) paged_extend_merge_kernel(con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int4* rec = reinterpret_cast<const int4*>(a.cuts + blockIdx.x + a.num_kv_heads);
   const int4 c0 = __ldcg(rec), c1 = __ldcg(rec + 1);
-  const int qo0 = c0.x, row0 = c0.y, nrows = c0.z, first = c0.w, count = c1.x, shares = c1.y, part = c1.z;
+  const int qo0 = c0.x, row0 = c0.y, nrows = c0.z, first = c0.w, shares = c1.x, part = c1.y;
   const int gmask = (1 << a.lg) - 1, Nq = a.num_kv_heads << a.lg;
   const size_t share_step = static_cast<size_t>(2) * a.num_kv_heads * ROWS * kPdRec;
   for (int i = blockIdx.y * WARPS + warp; ; i += kXtMergeSplit * WARPS) {
@@ -833,14 +870,14 @@ __global__ void __launch_bounds__(kXtMergeThreads) paged_extend_merge_kernel(con
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int U = 4;
-    for (int z0 = 0; z0 < count; z0 += U) {   // four states are requested together
+    for (int z0 = 0; z0 <= shares; z0 += U) {   // four states are requested together
       float2 ml[U];
       float4 o[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         ml[u] = make_float2(0.f, 0.f);
         o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (z0 + u < count) {
+        if (z0 + u <= shares) {
           const float* r = base + (z0 + u) * share_step +
                            (z0 + u == 0 && part ? static_cast<size_t>(a.num_kv_heads) * ROWS * kPdRec : 0);
           ml[u] = __ldcg(reinterpret_cast<const float2*>(r));
