@@ -284,15 +284,15 @@ __device__ __forceinline__ void ex_layout(const ExArgs& a, int w0, unsigned per,
 template <int QT, bool DENSE = false>
 struct Xt {
   static constexpr int kRows = 32 * QT;
-  static constexpr int kStages = QT == 4 ? 2 : 3;       // of the K ring and of the V ring
-  static constexpr int kSegs = QT == 2 ? 4 : 16;
+  static constexpr int kKStages = 3, kVStages = QT == 4 ? 2 : 3;   // of the rings
+  static constexpr int kSegs = QT == 1 ? 16 : 4;
   static constexpr int kRotWarps = DENSE ? 0 : 4;
   static constexpr int kThreads = 32 * (2 * QT + kRotWarps + 4);
   static constexpr int kQPanel = kRows * 128;           // Q: two 64-dim panels of [rows][128 B]
   static constexpr int kKOff = 2 * kQPanel;
-  static constexpr int kVOff = kKOff + kStages * kXtTileBytes;
-  static constexpr int kBarOff = kVOff + kStages * kXtTileBytes;
-  static constexpr int kBars = 5 * kStages + 7;
+  static constexpr int kVOff = kKOff + kKStages * kXtTileBytes;
+  static constexpr int kBarOff = kVOff + kVStages * kXtTileBytes;
+  static constexpr int kBars = 3 * kKStages + 2 * kVStages + 7;
   static constexpr int kTurnOff = (kBarOff + kBars * 8 + 8 + 15) / 16 * 16;
   static constexpr int kScratchOff = kTurnOff + 512;
   static constexpr int kSmem = kScratchOff + static_cast<int>(sizeof(ExScratch<kSegs>));
@@ -328,7 +328,7 @@ __device__ __forceinline__ uint64_t load_if(const void* const* at, bool yes) {
 template <typename T, int QT, bool DENSE>
 __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_extend_kernel(const __grid_constant__ ExArgs a) {
   using X = Xt<QT, DENSE>;
-  constexpr int ROWS = X::kRows, NS = X::kStages, ROTATORS = 32 * X::kRotWarps;
+  constexpr int ROWS = X::kRows, NK = X::kKStages, NV = X::kVStages, ROTATORS = 32 * X::kRotWarps;
   extern __shared__ __align__(1024) unsigned char xt_smem[];
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -362,10 +362,10 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
   const int Nq = a.num_kv_heads << a.lg, P = a.page_size;
 
   const uint32_t qs = sbase, ks0 = sbase + X::kKOff, vs0 = sbase + X::kVOff, bars = sbase + X::kBarOff;
-  const uint32_t k_raw = bars, k_full = k_raw + NS * 8, k_empty = k_full + NS * 8, v_full = k_empty + NS * 8, v_empty = v_full + NS * 8;
+  const uint32_t k_raw = bars, k_full = k_raw + NK * 8, k_empty = k_full + NK * 8, v_full = k_empty + NK * 8, v_empty = v_full + NV * 8;
   // two each, used by alternate tiles: a softmax warp may be a tile ahead of another, and looks at the completion of a tile
   // after it has handed on the next
-  const uint32_t s_full = v_empty + NS * 8, p_full = s_full + 16, o_done = s_full + 32;
+  const uint32_t s_full = v_empty + NV * 8, p_full = s_full + 16, o_done = s_full + 32;
   const uint32_t q_full = s_full + 48, tmem_slot = s_full + 56;
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(xt_smem + (tmem_slot - sbase));
   // roles: softmax warps w < 8 with w mod 4 < QT; of the others, in the order of their numbers, the rotators, a loader of K,
@@ -378,10 +378,12 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
   if (sc.count == 0) return;   // nothing left for this share (uniform over the CTA)
 
   if (tid == 0) {
-    for (int i = 0; i < NS; ++i) {
+    for (int i = 0; i < NK; ++i) {
       mbar_init(k_raw + i * 8, 32);
       mbar_init(k_full + i * 8, DENSE ? 32 : ROTATORS);
       mbar_init(k_empty + i * 8, 1);
+    }
+    for (int i = 0; i < NV; ++i) {
       mbar_init(v_full + i * 8, 32);
       mbar_init(v_empty + i * 8, 1);
     }
@@ -426,8 +428,8 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
               ss[k] = pack_f32x2(s0, sx);
             }
           }
-          const int st = g % NS;
-          pf_wait_role(k_raw + st * 8, (g / NS) & 1, a.err, dead);
+          const int st = g % NK;
+          pf_wait_role(k_raw + st * 8, (g / NK) & 1, a.err, dead);
           // row kr of a panel; rows STEP further on are swizzled alike
           uint32_t at = ks0 + st * kXtTileBytes + kr * 128 + ((c ^ (kr & 7)) << 4);
 #pragma unroll 1
@@ -480,6 +482,9 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
         const int row = 2 * i + (lane >> 4);
         dst[i] = ring + ((lane & 8) ? kXtPanel : 0) + row * 128 + (((lane & 7) ^ row) << 4);
       }
+      const int stages = role == 1 ? NK : NV;
+      int st = g % stages;                       // stage of the next tile
+      uint32_t phase = (g / stages - 1) & 1;     // of its last use
       bool bad_ptr = false;
       // eight keys lie in one page: lane e looks after the keys 8 e .. 8 e + 7 of the tile, a tile ahead of the copies
       const int e8 = (lane & 7) * 8;
@@ -503,8 +508,7 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
           const bool whole = __all_sync(0xffffffffu, ok) && key0 + kXtKeys <= nkeys;
           const uint64_t mine = ok ? base : 0;
           page = j + 1 < ntiles ? entry(sc.seg[seg], tile0 + j + 1) : next < count ? entry(sc.seg[next], sc.seg[next].tile0) : 0;
-          const int st = g % NS;
-          if (g >= NS) pf_wait_role(empty + st * 8, (g / NS - 1) & 1, a.err, dead);
+          if (g >= stages) pf_wait_role(empty + st * 8, phase, a.err, dead);
           if (dead) break;
           const uint32_t off = st * kXtTileBytes;
           if (whole) {
@@ -529,6 +533,10 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
             }
           }
           cp_async_arrive(full + st * 8);   // when this lane's copies have landed
+          if (++st == stages) {
+            st = 0;
+            phase ^= 1;
+          }
         }
       }
       cp_async_wait<0>();
@@ -542,8 +550,8 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
           const int ntiles = sc.seg[seg].ntiles;
           pf_wait_role(q_full, gs & 1, a.err, dead);
           for (int j = 0; j < ntiles; ++j, ++g) {
-            const int st = g % NS, sb = g & 1;
-            pf_wait_role(k_full + st * 8, (g / NS) & 1, a.err, dead);
+            const int st = g % NK, sb = g & 1;
+            pf_wait_role(k_full + st * 8, (g / NK) & 1, a.err, dead);
             if (DENSE) fence_proxy_async();   // K came by the loader's ordinary copies
             if (g >= 2) pf_wait_role(o_done + sb * 8, ((g >> 1) - 1) & 1, a.err, dead);   // P . V has read this S buffer
             tc_fence_after();
@@ -568,8 +576,8 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
         for (int seg = 0; seg < count; ++seg) {
           const int ntiles = sc.seg[seg].ntiles;
           for (int j = 0; j < ntiles; ++j, ++g) {
-            const int st = g % NS, sb = g & 1;
-            pf_wait_role(v_full + st * 8, (g / NS) & 1, a.err, dead);
+            const int st = g % NV, sb = g & 1;
+            pf_wait_role(v_full + st * 8, (g / NV) & 1, a.err, dead);
             fence_proxy_async();   // V came by the loader's ordinary copies
             pf_wait_role(p_full + sb * 8, (g >> 1) & 1, a.err, dead);
             tc_fence_after();
