@@ -41,12 +41,21 @@ struct ExPlan {
   size_t bytes;    // and of rotated keys
 };
 
+// Rows of a row tile, by the mean number of rows (new tokens x query heads per kv head) of a request.  A tile's rows cost
+// softmax work and queries; rows that do not fit one tile walk the keys again.  32 requests with contexts 512..4096, 32 / 8
+// heads, bf16, us with tiles of 32 / 64 / 128 rows, by rows per request:
+//   4 and 8  87 / 95 / 101    32  91 / 99 / 103    40  155 / 97 / 110    64  153 / 101 / 114    80  214 / 167 / 116
+// Keys rotated once in front (three more passes over them) or by every row tile that meets them, us, in place / in front, 32 / 8
+// heads, by rows per request:
+//   1 request on 16 k keys    256  67 / 69      384  81 / 77      512  95 / 85      1024  153 / 122    4096  489 / 333
+//   8 requests on 4 k keys    256  103 / 103    384  134 / 126    512  163 / 142    1024  282 / 230    4096  1052 / 798
 ExPlan extend_plan(int batch, int total_q, int total_pages, int page_size, int num_kv_heads, int group) {
   ExPlan p;
   const long long all_rows = static_cast<long long>(total_q) * group;
   const long long mean = (all_rows + batch - 1) / batch;
   p.qt = mean <= 32 ? 1 : mean <= 64 ? 2 : 4;
-  p.min_tiles = 4;
+  p.dense = mean > 256;
+  p.min_tiles = 4;   // (a share pays for its start: 18 us for 300 keys in shares of 4 tiles as of 8)
   const int rows = 32 * p.qt;
   // all the CTAs that are resident, but no more than the work can hold
   const long long key_tiles = static_cast<long long>(total_pages) * page_size / kXtKeys + batch;
@@ -54,7 +63,6 @@ ExPlan extend_plan(int batch, int total_q, int total_pages, int page_size, int n
   p.fits = (all_rows / rows + batch) * key_tiles < 0x7fffff00LL;
   p.shares = static_cast<int>(std::min<long long>(std::max(1, kXtCtasPerSm * kNumSMs / num_kv_heads), most));
   p.state = p.shares > 1 ? static_cast<size_t>(p.shares) * num_kv_heads * (sizeof(ExCut) + 2 * rows * kPdRec * sizeof(float)) : 0;
-  p.dense = p.qt == 4 && mean >= 256;
   p.bytes = p.state + (p.dense ? static_cast<size_t>(total_pages) * page_size * num_kv_heads * kPdDim * 2 : 0);
   return p;
 }

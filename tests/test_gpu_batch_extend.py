@@ -97,13 +97,24 @@ def test_far_positions_lose_nothing():
     _check(5, [70001], [3], 1, 4, 64, torch.float16)
 
 
-def test_uneven_batch_of_many_requests():
-    """More requests than the threads that look for a CTA's share of the work, one far longer than the rest."""
-    r = random.Random(9)
-    new = [r.randint(0, 4) for _ in range(300)]
+@pytest.mark.parametrize("requests,most,heads", [(300, 4, (2, 4)), (700, 3, (1, 8)), (3000, 2, (1, 1)), (700, 12, (1, 4)),
+                                                  (400, 30, (2, 4))])
+def test_uneven_batch_of_many_requests(requests, most, heads):
+    """More requests than a CTA looks at together and more row tiles in a share than are laid out at a time; many without
+    a new token, one far longer than the rest."""
+    r = random.Random(requests)
+    new = [r.choice([0, r.randint(0, most), most]) for _ in range(requests)]
     lens = [n + r.randint(0, 90) for n in new]
     lens[217] = 6000
-    _check(6, lens, new, 2, 4, 16, torch.bfloat16)
+    _check(requests, lens, new, *heads, 16, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,page", [((2, 4), 16), ((1, 8), 8), ((3, 2), 64), ((4, 1), 32)])
+def test_long_chunks_whose_keys_are_rotated_in_front(dtype, heads, page):
+    """Several row tiles per request: whole prompts, pieces of prompts, beside an empty request and one of a token."""
+    n = 1300 // heads[1]
+    _check(page, [n, n + 777, 0, 3 * n + 5, 64, n + 1], [n, n, 0, n + 3, 1, n], *heads, page, dtype)
 
 
 def test_large_scores():
