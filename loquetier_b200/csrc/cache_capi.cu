@@ -127,9 +127,9 @@ template <typename T>
 int launch_qk_bwd(const HeadNormArgs& a, void* dwq, void* dwk, cudaStream_t stream) {
   const bool norm = a.s[0].w != nullptr, rope = a.positions != nullptr;
   const dim3 grid(a.s[0].ctas + a.s[1].ctas, 1, 1);
-  if (!norm) return launch(qk_norm_rope_bwd_kernel<T, false, true>, grid, kHnThreads, 1, 0, stream, a);
-  const int rc = rope ? launch(qk_norm_rope_bwd_kernel<T, true, true>, grid, kHnThreads, 1, 0, stream, a)
-                      : launch(qk_norm_rope_bwd_kernel<T, true, false>, grid, kHnThreads, 1, 0, stream, a);
+  if (!norm) return launch(qk_norm_rope_bwd_kernel<T, false, true>, grid, kHnThreads, 1, kHnSmem, stream, a);
+  const int rc = rope ? launch(qk_norm_rope_bwd_kernel<T, true, true>, grid, kHnThreads, 1, kHnSmem, stream, a)
+                      : launch(qk_norm_rope_bwd_kernel<T, true, false>, grid, kHnThreads, 1, kHnSmem, stream, a);
   if (rc != SMLM_OK) return rc;
   return launch(head_norm_dw_kernel<T>, dim3(2 * kPdDim / 8, 1, 1), 256, 1, 0, stream, dwq, dwk, a.partial, a.s[0].ctas,
                 static_cast<int>(grid.x));

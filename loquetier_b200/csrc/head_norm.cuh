@@ -149,12 +149,41 @@ __global__ void __launch_bounds__(kHnThreads, 3) qk_norm_rope_kernel(const __gri
                                   4 * st.splits, w, cs, sn, c, hl, a.eps);
 }
 
-// Warps walk over (token, share of its heads) with a fixed stride, four heads at a time with the next four requested
-// before the current ones are worked on, and keep their share of dw in fp32 registers; the CTA adds its warps' in warp order
-// and parks one row, which head_norm_dw_kernel adds in row order: the same result each time.
+constexpr int kHnAhead = 3;                          // fours of heads on their way per warp
+constexpr int kHnStage = 4 * 512;                    // of four heads: gradient and input, two halves of a head's row each
+constexpr int kHnRing = (kHnAhead + 1) * kHnStage;
+constexpr int kHnSmem = kHnWarps * kHnRing;
+
+// eight 16-bit values as four packed pairs of fp32, and back
+template <typename T>
+__device__ __forceinline__ void pairs8(const uint4& u, uint64_t* f) {
+  const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y), c = unpack2<T>(u.z), d = unpack2<T>(u.w);
+  f[0] = pack_f32x2(a.x, a.y);
+  f[1] = pack_f32x2(b.x, b.y);
+  f[2] = pack_f32x2(c.x, c.y);
+  f[3] = pack_f32x2(d.x, d.y);
+}
+template <typename T>
+__device__ __forceinline__ uint4 packed8(const uint64_t* f) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    unpack_f32x2(f[i], a, b);
+    r[i] = pack2<T>(a, b);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Warps walk over (token, share of its heads) with a fixed stride, four heads at a time, and keep their share of dw in fp32
+// registers; the CTA adds its warps' in warp order and parks one row, which head_norm_dw_kernel adds in row order: the same
+// result each time.  Bound by HBM, so by what is in flight: a warp has the next kHnAhead fours on their way, as asynchronous
+// copies into a ring of its own in shared memory (a lane reads back what it copied: no barrier).  Measured, 8192 tokens of
+// 32 / 8 heads, bf16 (252 MB):
 template <typename T, bool NORM, bool ROPE>
 __global__ void __launch_bounds__(kHnThreads, 2) qk_norm_rope_bwd_kernel(const __grid_constant__ HeadNormArgs a) {
-  __shared__ float red[NORM ? kHnWarps : 1][kPdDim];
+  extern __shared__ __align__(16) unsigned char hn_ring[];
+  __shared__ __align__(8) float red[NORM ? kHnWarps : 1][kPdDim];
   __shared__ __align__(16) float freq[ROPE ? 128 : 4];
   const int lane = threadIdx.x & 31, c = lane & 7, hl = lane >> 3, warp = threadIdx.x >> 5;
   if (ROPE) {
@@ -166,88 +195,123 @@ __global__ void __launch_bounds__(kHnThreads, 2) qk_norm_rope_bwd_kernel(const _
   const bool keys = blockIdx.x >= a.s[0].ctas;
   const HeadNormStream& st = a.s[keys];
   const int heads = st.heads, step = 4 * st.splits;
-  float w[16], dw[16], cs[8], sn[8];
-  load_weight<T, NORM>(st.w, c, w);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) dw[i] = 0.f;
+  uint64_t w[8], dw[8] = {}, cs[4], sn[4];   // pairs
+  if (NORM) {
+    pairs8<T>(__ldg(static_cast<const uint4*>(st.w) + c), w);
+    pairs8<T>(__ldg(static_cast<const uint4*>(st.w) + 8 + c), w + 4);
+  }
   // (few tokens are split, many are not: the numbers of units stay below 2^32)
   const unsigned units = static_cast<unsigned>(a.T) * st.splits, stride = static_cast<unsigned>(st.ctas) * kHnWarps;
   unsigned unit = (blockIdx.x - (keys ? a.s[0].ctas : 0)) * kHnWarps + warp;
   int t = static_cast<int>(unit / st.splits), h0 = static_cast<int>(unit % st.splits) * 4;   // where the loads are
-  uint4 nx[2], ng[2];
-  auto request = [&]() {
+  const uint32_t ring = smem_u32(hn_ring) + warp * kHnRing + lane * 16;
+  auto request = [&](int stage) {
     const int h = h0 + hl;
-    nx[0] = nx[1] = ng[0] = ng[1] = make_uint4(0u, 0u, 0u, 0u);
-    if (unit < units && h < heads) {
-      const T* g = static_cast<const T*>(st.g) + (static_cast<size_t>(t) * heads + h) * kPdDim + c * 8;
-      ng[0] = __ldcs(reinterpret_cast<const uint4*>(g));
-      ng[1] = __ldcs(reinterpret_cast<const uint4*>(g + 64));
-      if (NORM) {
-        const T* x = static_cast<const T*>(st.x) + t * st.stride + h * kPdDim + c * 8;
-        nx[0] = __ldcs(reinterpret_cast<const uint4*>(x));
-        nx[1] = __ldcs(reinterpret_cast<const uint4*>(x + 64));
-      }
+    const bool ok = unit < units && h < heads;
+    const T* g = static_cast<const T*>(st.g);
+    if (ok) g += (static_cast<size_t>(t) * heads + h) * kPdDim + c * 8;
+    const uint32_t dst = ring + stage * kHnStage;
+    cp_async16(dst, g, ok);
+    cp_async16(dst + 512, g + (ok ? 64 : 0), ok);
+    if (NORM) {
+      const T* x = static_cast<const T*>(st.x);
+      if (ok) x += t * st.stride + h * kPdDim + c * 8;
+      cp_async16(dst + 1024, x, ok);
+      cp_async16(dst + 1536, x + (ok ? 64 : 0), ok);
+    }
+    cp_async_commit();
+  };
+  auto advance = [&](unsigned& u, int& tok, int& head) {
+    head += step;
+    if (head >= heads) {
+      u += stride;
+      tok = static_cast<int>(u / st.splits);
+      head = static_cast<int>(u % st.splits) * 4;
     }
   };
-  request();
+  unsigned cu = unit;   // where the work is
+  int ct = t, ch = h0, stage = 0;
+#pragma unroll
+  for (int i = 0; i < kHnAhead; ++i) {
+    request(i);
+    advance(unit, t, h0);
+  }
   int at = -1;   // the token that the cosines and sines belong to
-  while (unit < units) {   // uniform over the warp
-    const int h = h0 + hl, tok = t;
-    float dp[8], dq[8], p[8], q[8];   // the gradient in front of the rotation, and the input
-    unpack8<T>(ng[0], dp);
-    unpack8<T>(ng[1], dq);
-    if (NORM) {
-      unpack8<T>(nx[0], p);
-      unpack8<T>(nx[1], q);
+  while (cu < units) {   // uniform over the warp
+    const int h = ch + hl, tok = ct;
+    const int free_stage = stage == 0 ? kHnAhead : stage - 1;   // of the four before this one
+    request(free_stage);
+    advance(unit, t, h0);
+    cp_async_wait<kHnAhead>();
+    // pairs of neighbouring dimensions, [0..3] of the lane's eight and [4..7] of their partners: the gradient in front of
+    // the rotation, and the input
+    uint64_t d[8], x[8];
+    const unsigned char* from = hn_ring + warp * kHnRing + stage * kHnStage + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      pairs8<T>(*reinterpret_cast<const uint4*>(from + i * 512), d + 4 * i);
+      if (NORM) pairs8<T>(*reinterpret_cast<const uint4*>(from + 1024 + i * 512), x + 4 * i);
     }
-    h0 += step;
-    if (h0 >= heads) {
-      unit += stride;
-      t = static_cast<int>(unit / st.splits);
-      h0 = static_cast<int>(unit % st.splits) * 4;
-    }
-    request();
+    stage = stage == kHnAhead ? 0 : stage + 1;
+    advance(cu, ct, ch);
     if (ROPE && tok != at) {
-      token_rotation<ROPE>(a, freq, tok, c, cs, sn);
+      float c8[8], s8[8];
+      token_rotation<ROPE>(a, freq, tok, c, c8, s8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cs[i] = pack_f32x2(c8[2 * i], c8[2 * i + 1]);
+        sn[i] = pack_f32x2(s8[2 * i], s8[2 * i + 1]);
+      }
       at = tok;
     }
+    constexpr uint64_t kNeg2 = 0x8000000080000000ull;   // flips the sign of both halves
     if (ROPE) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float r = dp[i] * cs[i] + dq[i] * sn[i];
-        dq[i] = dq[i] * cs[i] - dp[i] * sn[i];
-        dp[i] = r;
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t r = fma_f32x2(d[i], cs[i], mul_f32x2(d[4 + i], sn[i]));
+        d[4 + i] = fma_f32x2(d[4 + i], cs[i], mul_f32x2(d[i], sn[i] ^ kNeg2));
+        d[i] = r;
       }
     }
     if (NORM) {
-      float ss = 0.f, dot = 0.f;
+      uint64_t ss2 = 0ull, dot2 = 0ull, wd[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ss += p[i] * p[i] + q[i] * q[i];
-        dot += w[i] * dp[i] * p[i] + w[8 + i] * dq[i] * q[i];
+        ss2 = fma_f32x2(x[i], x[i], ss2);
+        wd[i] = mul_f32x2(w[i], d[i]);
+        dot2 = fma_f32x2(wd[i], x[i], dot2);
       }
-      const float s = rsqrtf(sum8(ss) * (1.0f / kPdDim) + a.eps);
-      const float coef = sum8(dot) * s * s * (1.0f / kPdDim);
+      float u, v;
+      unpack_f32x2(ss2, u, v);
+      const float s = rsqrtf(sum8(u + v) * (1.0f / kPdDim) + a.eps);
+      unpack_f32x2(dot2, u, v);
+      const float coef = -sum8(u + v) * s * s * (1.0f / kPdDim);
+      const uint64_t s2 = pack_f32x2(s, s), coef2 = pack_f32x2(coef, coef);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        dw[i] += p[i] * s * dp[i];
-        dw[8 + i] += q[i] * s * dq[i];
-        dp[i] = s * (w[i] * dp[i] - p[i] * coef);
-        dq[i] = s * (w[8 + i] * dq[i] - q[i] * coef);
+        const uint64_t xs = mul_f32x2(x[i], s2);
+        dw[i] = fma_f32x2(xs, d[i], dw[i]);
+        d[i] = fma_f32x2(xs, coef2, mul_f32x2(wd[i], s2));
       }
     }
     if (h < heads) {
       T* dx = static_cast<T*>(st.y) + (static_cast<size_t>(tok) * heads + h) * kPdDim + c * 8;
-      __stcs(reinterpret_cast<uint4*>(dx), pack8<T>(dp));
-      __stcs(reinterpret_cast<uint4*>(dx + 64), pack8<T>(dq));
+      __stcs(reinterpret_cast<uint4*>(dx), packed8<T>(d));
+      __stcs(reinterpret_cast<uint4*>(dx + 64), packed8<T>(d + 4));
     }
   }
+  cp_async_wait<0>();
   if (NORM) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
+      float u, v;
+      unpack_f32x2(dw[i], u, v);
 #pragma unroll
-      for (int d = 8; d < 32; d <<= 1) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], d);
-      if (hl == 0) red[warp][(i >> 3) * 64 + c * 8 + (i & 7)] = dw[i];
+      for (int m = 8; m < 32; m <<= 1) {
+        u += __shfl_xor_sync(0xffffffffu, u, m);
+        v += __shfl_xor_sync(0xffffffffu, v, m);
+      }
+      if (hl == 0) *reinterpret_cast<float2*>(&red[warp][(i >> 2) * 64 + c * 8 + (i & 3) * 2]) = make_float2(u, v);
     }
     __syncthreads();
     if (threadIdx.x < kPdDim) {

@@ -856,8 +856,20 @@ __global__ void __launch_bounds__(128) extend_rotate_kernel(const __grid_constan
 // Merges the states of the row tiles that are cut, in the order of the keys.  grid: ((shares - 1) * Nkv, kXtMergeSplit); a
 // CTA stands for the cut at the start of a share and serves some of the rows of the tile that it goes through, a warp a row
 // at a time, a lane four dimensions.
+// adds one softmax state to another; an empty one (no weight) carries no information
+__device__ __forceinline__ void add_state(float m1, float l1, const float4& o1, float& m, float& l, float4& acc) {
+  if (l1 == 0.f) return;
+  const float mn = fmaxf(m, m1), w0 = l == 0.f ? 0.f : exp2f(m - mn), w1 = exp2f(m1 - mn);
+  m = mn;
+  l = l * w0 + l1 * w1;
+  acc.x = acc.x * w0 + o1.x * w1;
+  acc.y = acc.y * w0 + o1.y * w1;
+  acc.z = acc.z * w0 + o1.z * w1;
+  acc.w = acc.w * w0 + o1.w * w1;
+}
+
 constexpr int kXtMergeThreads = 256;
-constexpr int kXtMergeSplit = 2;
+constexpr int kXtMergeSplit = 2;   // (four to eight times as many CTAs of fewer rows measured the same or slower)
 
 template <typename T, int QT>
 __global__ void __launch_bounds__(kXtMergeThreads) paged_extend_merge_kernel(const __grid_constant__ ExArgs a) {
@@ -871,48 +883,68 @@ __global__ void __launch_bounds__(kXtMergeThreads) paged_extend_merge_kernel(con
   const int qo0 = c0.x, row0 = c0.y, nrows = c0.z, first = c0.w, shares = c1.x, part = c1.y;
   const int gmask = (1 << a.lg) - 1, Nq = a.num_kv_heads << a.lg;
   const size_t share_step = static_cast<size_t>(2) * a.num_kv_heads * ROWS * kPdRec;
-  for (int i = blockIdx.y * WARPS + warp; ; i += kXtMergeSplit * WARPS) {
-    const int row = i * shares + share - first - 1;
-    if (nrows == 0 || row >= nrows) break;
+  if (nrows == 0) return;
+  const int count = shares + 1;
+  // the states z0 .. z1 - 1 of a row, in order, added to (m, l, acc)
+  auto add_states = [&](int row, int z0, int z1, float& m, float& l, float4& acc) {
     const float* base = a.partial + ((static_cast<size_t>(first) * 2 * a.num_kv_heads + kvh) * ROWS + row) * kPdRec;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int U = 4;
-    for (int z0 = 0; z0 <= shares; z0 += U) {   // four states are requested together
+    for (; z0 < z1; z0 += U) {   // four states are requested together
       float2 ml[U];
       float4 o[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         ml[u] = make_float2(0.f, 0.f);
         o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (z0 + u <= shares) {
+        if (z0 + u < z1) {
           const float* r = base + (z0 + u) * share_step +
                            (z0 + u == 0 && part ? static_cast<size_t>(a.num_kv_heads) * ROWS * kPdRec : 0);
           ml[u] = __ldcg(reinterpret_cast<const float2*>(r));
           o[u] = __ldcg(reinterpret_cast<const float4*>(r + 4) + lane);
         }
       }
-      float mn = m;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (ml[u].y != 0.f) mn = fmaxf(mn, ml[u].x);   // an empty state carries no information
-      const float w0 = l != 0.f ? exp2f(m - mn) : 0.f;
-      m = mn;
-      l *= w0;
-      acc.x *= w0; acc.y *= w0; acc.z *= w0; acc.w *= w0;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (ml[u].y != 0.f) {
-          const float wt = exp2f(ml[u].x - m);
-          l += ml[u].y * wt;
-          acc.x += o[u].x * wt; acc.y += o[u].y * wt; acc.z += o[u].z * wt; acc.w += o[u].w * wt;
-        }
-      }
+      for (int u = 0; u < U; ++u) add_state(ml[u].x, ml[u].y, o[u], m, l, acc);
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+  };
+  auto write_row = [&](int row, float l, const float4& acc) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;   // no keys: zeros; a NaN stays one
     const int rr = row0 + row;
     T* op = static_cast<T*>(a.o) + (static_cast<size_t>(qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim;
     reinterpret_cast<uint2*>(op)[lane] = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  };
+  if (count <= 2 * WARPS) {   // a warp per row
+    for (int i = blockIdx.y * WARPS + warp; ; i += kXtMergeSplit * WARPS) {
+      const int row = i * shares + share - first - 1;
+      if (row >= nrows) return;
+      float m = -INFINITY, l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      add_states(row, 0, count, m, l, acc);
+      write_row(row, l, acc);
+    }
+  }
+  // few rows of many states (a long cache): the CTA's warps take a run of a row's states each
+  __shared__ float4 s_acc[WARPS][32];
+  __shared__ float2 s_ml[WARPS];
+  const int run = (count + WARPS - 1) / WARPS;
+  for (int i = blockIdx.y; ; i += kXtMergeSplit) {
+    const int row = i * shares + share - first - 1;   // the same in every warp
+    if (row >= nrows) return;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    add_states(row, warp * run, min(count, (warp + 1) * run), m, l, acc);
+    s_acc[warp][lane] = acc;
+    if (lane == 0) s_ml[warp] = make_float2(m, l);
+    __syncthreads();
+    if (warp == 0) {
+      m = -INFINITY;
+      l = 0.f;
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < WARPS; ++v) add_state(s_ml[v].x, s_ml[v].y, s_acc[v][lane], m, l, acc);
+      write_row(row, l, acc);
+    }
+    __syncthreads();
   }
 }
 
