@@ -100,8 +100,9 @@ int smlm_b200_init_kv(const void* const* kv_ptrs, const int32_t* kv_indptr, cons
 
 /* ---- operators around a cache that several continuations share -------------------------------------- */
 
-/* Bytes of the workspace of smlm_b200_batch_extend for a batch of these sizes (0: none is needed).  Its contents
- * matter neither before nor after a call; launches that may overlap in time must not share one. */
+/* Bytes of the workspace of smlm_b200_batch_extend for a batch of these sizes (0: none is needed): softmax states of row
+ * tiles that are cut and, for chunks of more than 256 rows (new tokens x query heads per kv head) per request, a rotated copy of the
+ * batch's keys.  Its contents matter neither before nor after a call; launches that may overlap in time must not share one. */
 size_t smlm_b200_batch_extend_workspace_bytes(int batch_size, int total_q, int total_pages, int page_size,
                                               int num_qo_heads, int num_kv_heads);
 
@@ -110,9 +111,11 @@ size_t smlm_b200_batch_extend_workspace_bytes(int batch_size, int total_q, int t
  * head_dim], 16-byte aligned), n_b >= 0 of them; its query i stands at position L_b - n_b + i and sees the keys up to its own:
  *   o[i, h] = softmax( rope(q[i, h], pos_i) . rope(K_b[0..pos_i, h / group])^T / sqrt(head_dim) ) . V_b[0..pos_i]
  * What smlm_b200_batch_prefill computes, for chunks that are short against their cache: the pages are read in place, and
- * long caches are cut into ranges of keys so that a few new tokens fill the machine.  The ranges follow from the lengths
- * on the device alone: the same batch gives the same result, whatever its page table's length.  Rows of no request are left
- * as they were; a row that sees no key is zeros.  Status word: bit 1 also where a request has more queries than keys. */
+ * long caches are spread over the machine so that a few new tokens fill it.  The cuts follow from the lengths on the device
+ * alone: the same batch gives the same result, whatever its page table's length.  Rows of no request are left
+ * as they were; a row that sees no key is zeros.  Angles are formed to 2^-40 turns for positions below 2^24.  A key or value that
+ * is not finite may reach every new token of its request, no other request.  Status word: bit 1 also where a request has more
+ * queries than keys; value 8: a bounded wait inside the kernel gave up (the output is then not valid). */
 int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, const void* const* kv_ptrs,
                            const int32_t* kv_indptr, const int32_t* last_page_offset, void* workspace,
                            size_t workspace_bytes, int* status_word, int batch_size, int total_q, int total_pages,

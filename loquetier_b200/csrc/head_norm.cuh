@@ -125,7 +125,8 @@ __device__ __forceinline__ void load_weight(const void* w, int c, float (&f)[16]
   }
 }
 
-// One warp per (token, share of its heads).  Measured, 8192 tokens of 32 / 8 heads, bf16 (168 MB): see the backward pass.
+// One warp per (token, share of its heads).  Measured, 8192 tokens of 32 / 8 heads, bf16 (168 MB, 26 us at the copy rate):
+// 31 us; 37 with both sets of weights in registers (two CTAs per SM instead of three).
 template <typename T, bool NORM, bool ROPE>
 __global__ void __launch_bounds__(kHnThreads, 3) qk_norm_rope_kernel(const __grid_constant__ HeadNormArgs a) {
   __shared__ __align__(16) float freq[ROPE ? 128 : 4];
@@ -179,7 +180,8 @@ __device__ __forceinline__ uint4 packed8(const uint64_t* f) {
 // registers; the CTA adds its warps' in warp order and parks one row, which head_norm_dw_kernel adds in row order: the same
 // result each time.  Bound by HBM, so by what is in flight: a warp has the next kHnAhead fours on their way, as asynchronous
 // copies into a ring of its own in shared memory (a lane reads back what it copied: no barrier).  Measured, 8192 tokens of
-// 32 / 8 heads, bf16 (252 MB):
+// 32 / 8 heads, bf16 (252 MB, 39 us at the copy rate): 82 us with both sets of weights and gradients in registers (one CTA
+// per SM), 50 with one stream per CTA and the next four heads requested ahead, 48 with the ring and packed arithmetic.
 template <typename T, bool NORM, bool ROPE>
 __global__ void __launch_bounds__(kHnThreads, 2) qk_norm_rope_bwd_kernel(const __grid_constant__ HeadNormArgs a) {
   extern __shared__ __align__(16) unsigned char hn_ring[];
@@ -367,7 +369,8 @@ struct NormAppendArgs {
   float eps;
 };
 
-// One warp per (token, share of its heads).
+// One warp per (token, share of its heads).  Measured: 10622 tokens of 32 / 8 heads in 12 prompts, fp16 (261 MB, 40 us at the
+// copy rate): 39 us; 64 single tokens: 6 us, latency.
 template <typename T>
 __global__ void __launch_bounds__(kHnThreads) norm_append_kernel(const NormAppendArgs a) {
   const int lane = threadIdx.x & 31, c = lane & 7, hl = lane >> 3;

@@ -3,7 +3,8 @@
 //
 // A page is [layers, 2, kv_heads, page_size, 128]: its first e entries are layers * 2 * kv_heads runs of e * 256 bytes,
 // page_size * 256 bytes apart.  Bound by HBM: every byte is read once and written once, eight 16-byte loads of a thread in
-// flight before its first store.
+// flight before its first store.  Measured: 280 pages of 2 MB 167 us (7.0 TB/s read and written), the filled parts of 24 last
+// pages to four continuations each (113 MB, 17 us at the copy rate) 20.5 us; 23.2 with a division per 16 bytes.
 #pragma once
 #include "paged_kv.cuh"
 

@@ -18,14 +18,31 @@
 //   O[128, 128] += P . V_tile      A = P in tensor memory, B = V MN-major as the cache stores it
 //
 // The products and the softmax are those of the prefill kernel (paged_prefill.cuh).  What differs is where the tiles come
-// from: here loader warps fetch K and V from the pages themselves with 16-byte asynchronous copies, straight into the
-// swizzled places the products read, and rotate the keys in place.  A loader thread has eight frequencies (dimensions
-// 8 c .. 8 c + 7 and their partners) and a fixed distance between its keys, so its cosines and sines go on from key to key
-// by one turn.  It waits for its own copies only, and runs ahead across row tiles and requests.
+// from: that kernel has the batch's cache copied into a dense workspace first, three times the bytes.  Here two warps, one for K
+// and one for V, fetch the tiles from the pages themselves with 16-byte asynchronous copies, straight into the swizzled
+// places the products read, and run ahead across row tiles and requests; four warps rotate the keys in place.  A rotator thread
+// has eight frequencies (dimensions 8 c .. 8 c + 7 and their partners) and a fixed distance between its keys, so its cosines
+// and sines go on from key to key by one turn and are computed afresh every 16 tiles, from angles good to 2^-40 turns.
+// Chunks of several row tiles would rotate every key several times: for them the keys are rotated once, in front, into a
+// dense copy (DENSE; the values stay where they are).
 //
 // The products always have 128 rows; what lies behind the tile's rows in shared memory feeds accumulator lanes that nobody
-// reads.  Softmax warps are those whose tensor-memory lanes hold the tile's rows, the loaders and the two issuers the others.
-// Every wait is bounded.
+// reads.  Softmax warps are those whose tensor-memory lanes hold the tile's rows, and warps of an empty quarter only pass
+// hand-offs on.  Every wait is bounded.
+//
+// Rounded to 16 bits, as the operands of the products: rotated queries and keys and the softmax weights; with the result's own
+// rounding the error against 64 bits is 3.3e-3 (bf16) and 4.1e-4 (fp16) of the result, where the result's rounding alone is
+// 1.7e-3 and 2.1e-4.  Keeping the lower halves too (products of twice the depth) would take the shared memory of a stage
+// of the rings and half of the tensor cores' time again.  Scores, maxima, sums and parked states are fp32.
+//
+// What bounds it (32 / 8 heads, B200).  32 requests, 512..4096 keys, 4 to 8 new tokens (285 MB, 44 us at the copy rate), 82 us a
+// pass: the launch 76, of which 6 are the search for the share and cold instructions, 5 the first tile, and the loop runs at
+// about the rate the pages arrive; the merge 5.  One request, 65 k keys, 17 tokens (269 MB): 85 us.  With 128 rows per tile the
+// loop is bound by issue slots (52 % used): of about 3400 warp instructions per tile, 1500 rotate, 1600 are the softmax's.
+// History on the first: one CTA per (row tile, range of keys) 146 us (CTAs of unequal length); even shares 100; roles whose
+// registers fit (spills in the loaders' loop) 94; copies and rotation in warps of their own 91; descriptors formed by one
+// addition, one barrier fewer, waits that sleep 84; key tiles counted exactly 82.  Waits that spin cost 5-15 % (they take
+// issue slots), eight rotator warps measured the same as four, mma.sync with 8, 16 or 32 rows per tile 130-166 us.
 #pragma once
 #include "paged_prefill.cuh"
 #include "rms_norm.cuh"
