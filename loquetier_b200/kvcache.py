@@ -71,6 +71,18 @@ class KvPool:
         self._allocated[page.data_ptr()] = page
         return page
 
+    def alloc_pages(self, n: int) -> List[torch.Tensor]:
+        """``n`` pages, or none where the memory does not suffice."""
+        pages = []
+        try:
+            for _ in range(n):
+                pages.append(self.alloc_page())
+        except BaseException:
+            for page in pages:
+                self.free_page(page)
+            raise
+        return pages
+
     def free_page(self, page: torch.Tensor) -> None:
         """Gives up one hold of the page; the last one makes it free."""
         ptr = page.data_ptr()
@@ -250,7 +262,7 @@ class KvCache:
         if n < 0:
             raise ValueError("n must be non-negative")
         need = -(-(self._seqlen + n) // self._pool.page_len) - len(self._pages)
-        new = [self._pool.alloc_page() for _ in range(need)]
+        new = self._pool.alloc_pages(need)
         self._pages.extend(new)
         self._ptrs.extend([p.data_ptr() for p in new])
         self._seqlen += n
@@ -268,7 +280,11 @@ class KvCache:
         if entries and pool.page_holders(self._pages[npages - 1]) > 1:
             refuse_capture(self._pages[npages - 1], "KvCache.truncate into a shared page")
             own = pool.alloc_page()
-            copy_pages(pool, *_page_tables(pool.device, [own], [self._pages[npages - 1]], [entries]))
+            try:
+                copy_pages(pool, *_page_tables(pool.device, [own], [self._pages[npages - 1]], [entries]))
+            except BaseException:
+                pool.free_page(own)
+                raise
         for page in self._pages[npages - (own is not None):]:
             pool.free_page(page)
         if own is not None:
@@ -311,10 +327,8 @@ def fork_caches(caches: Sequence[KvCache], copies: int = 1) -> List[List[KvCache
     partial = [c for c in caches if c.seqlen % pool.page_len]
     if partial and copies:
         refuse_capture(partial[0].pages[-1], "a fork that copies pages")
-    tails = []
+    tails = pool.alloc_pages(len(partial) * copies)
     try:
-        for _ in range(len(partial) * copies):
-            tails.append(pool.alloc_page())
         if tails:
             src = [c.pages[-1] for c in partial for _ in range(copies)]
             entries = [c.seqlen % pool.page_len for c in partial for _ in range(copies)]
@@ -566,8 +580,8 @@ def batch_extend(q: torch.Tensor, qo_indptr: torch.Tensor, kv: BatchedKvCache, b
     _chk_cuda_contig(qo_indptr, "qo_indptr", 1)
     if qo_indptr.dtype != torch.int32 or qo_indptr.numel() != kv.last_page_offset.numel() + 1:
         raise RuntimeError(f"qo_indptr must hold {kv.last_page_offset.numel() + 1} int32 values")
-    if q.dtype != kv.pool.dtype:
-        raise RuntimeError(f"q must be {kv.pool.dtype} like the cache")
+    if q.dtype != kv.pool.dtype or q.size(2) != kv.pool.head_dim:
+        raise RuntimeError(f"q must be {kv.pool.dtype} with heads of {kv.pool.head_dim} like the cache")
     _chk_same_device(q, qo_indptr=qo_indptr, kv=kv.ptrs)
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     return batch_extend_into(o, q, qo_indptr, kv.ptrs, kv.indptr, kv.last_page_offset, kv.pool.num_layers, layer_idx,
