@@ -114,7 +114,7 @@ size_t smlm_b200_batch_extend_workspace_bytes(int batch_size, int total_q, int t
  * long caches are spread over the machine so that a few new tokens fill it.  The cuts follow from the lengths on the device
  * alone: the same batch gives the same result, whatever its page table's length.  Rows of no request are left
  * as they were; a row that sees no key is zeros.  Angles are formed to 2^-40 turns for positions below 2^24.  A key or value that
- * is not finite may reach every new token of its request, no other request.  Status word: bit 1 also where a request has more
+ * is not finite reaches the tokens that see it and no others.  o must not overlap q.  Status word: bit 1 also where a request has more
  * queries than keys; value 8: a bounded wait inside the kernel gave up (the output is then not valid). */
 int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, const void* const* kv_ptrs,
                            const int32_t* kv_indptr, const int32_t* last_page_offset, void* workspace,

@@ -218,6 +218,38 @@ def test_bad_tables_are_reported_not_followed():
     R.check_extend(o[3:5], want[3:5], bound[3:5], torch.bfloat16, "the sound request beside a bad one")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,length,group,far", [(5, 300, 4, 1), (40, 300, 1, 7), (70, 2000, 8, 30), (200, 200, 4, 100), (3, 9000, 8, 2)])
+def test_what_is_not_finite_reaches_only_those_who_see_it(dtype, new, length, group, far):
+    """NaN and infinities among the new tokens' keys and values: earlier tokens are as if they were not there."""
+    pool, args, starts, dense = _batch(50 + new, [length, 77], [new, 3], 2, group, 16, dtype)
+    clean = _run(args)
+    at = length - far                                   # the token whose value is spoilt, seen from query new - far on
+    def spoil(which, position, head, dims, value):
+        page = args["kv_ptrs"].tolist().index(args["kv_ptrs"][position // 16].item())
+        ids = [i for i in range(pool.size(0)) if pool[i].data_ptr() == args["kv_ptrs"][page].item()]
+        pool[ids[0], LAYER, which, head, position % 16, dims] = value
+    spoil(1, at, 0, slice(3, 5), float("nan"))
+    spoil(1, at, 1, slice(127, 128), float("-inf"))
+    if far > 1:
+        spoil(1, length - 1, 1, slice(0, 1), float("inf"))
+        spoil(0, length - 1, 0, slice(9, 10), float("nan"))
+    o = _run(args)
+    first = new - far
+    assert torch.equal(o[:first], clean[:first]) and torch.equal(o[new:], clean[new:])
+    seen, G = o[first:new], group
+    assert torch.isnan(seen[:, :G, 3:5]).all() and (seen[:, G:, 127] == float("-inf")).all()
+    last = new - 1
+    keep = torch.ones(128, dtype=torch.bool, device=DEV)
+    keep[3:5] = False
+    rows = slice(first, last if far > 1 else new)
+    assert torch.equal(o[rows, :G][..., keep], clean[rows, :G][..., keep])
+    assert torch.equal(o[rows, G:, :127], clean[rows, G:, :127])
+    if far > 1:
+        assert torch.isnan(o[last, :G]).all() and (o[last, G:, 0] == float("inf")).all()
+        assert torch.equal(o[last, G:, 1:127], clean[last, G:, 1:127])
+
+
 def test_more_queries_than_keys():
     """Rows that see no key are zeros, the others as the definition has them; the status word tells."""
     pool, args, starts, dense = _batch(41, [3, 30], [3, 4], 2, 4, 16, torch.float16)
