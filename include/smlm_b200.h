@@ -373,8 +373,8 @@ size_t smlm_b200_qk_norm_rope_bwd_workspace_bytes(int T, int num_qo_heads, int n
 
 /* Backward of the above from the gradients gq and gk of yq and yk (contiguous):
  *   dn = g rotated back      dw = sum over rows and heads of x s dn      dx = s (w dn - x s^2 mean(w dn x)),  s the rsqrt
- * dq and dk contiguous; dwq and dwk [head_dim] in `dtype` (NULL without weights), summed in fp32 in a fixed order.  T must be
- * positive. */
+ * dq and dk contiguous; dwq and dwk [head_dim] in `dtype`, summed in fp32 in a fixed order (both NULL without weights or where
+ * these are not trained: no workspace then).  T must be positive. */
 int smlm_b200_qk_norm_rope_bwd(void* dq, void* dk, void* dwq, void* dwk, const void* gq, const void* gk, const void* q,
                                const void* k, const void* wq, const void* wk, const void* positions, void* workspace,
                                size_t workspace_bytes, long long q_stride, long long k_stride, int T, int num_qo_heads,

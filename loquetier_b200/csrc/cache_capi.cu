@@ -130,7 +130,7 @@ int launch_qk_bwd(const HeadNormArgs& a, void* dwq, void* dwk, cudaStream_t stre
   if (!norm) return launch(qk_norm_rope_bwd_kernel<T, false, true>, grid, kHnThreads, 1, kHnSmem, stream, a);
   const int rc = rope ? launch(qk_norm_rope_bwd_kernel<T, true, true>, grid, kHnThreads, 1, kHnSmem, stream, a)
                       : launch(qk_norm_rope_bwd_kernel<T, true, false>, grid, kHnThreads, 1, kHnSmem, stream, a);
-  if (rc != SMLM_OK) return rc;
+  if (rc != SMLM_OK || dwq == nullptr) return rc;
   return launch(head_norm_dw_kernel<T>, dim3(2 * kPdDim / 8, 1, 1), 256, 1, 0, stream, dwq, dwk, a.partial, a.s[0].ctas,
                 static_cast<int>(grid.x));
 }
@@ -179,8 +179,8 @@ int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, con
   if (group != 1 && group != 2 && group != 4 && group != 8) return SMLM_ERR_NO_KERNEL;
   if (batch_size == 0 || total_q == 0) return SMLM_OK;
   if (o == nullptr || q == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || last_page_offset == nullptr ||
-      (kv_ptrs == nullptr && total_pages > 0))
-    return SMLM_ERR_INVALID_ARGUMENT;
+      (kv_ptrs == nullptr && total_pages > 0) || o == q)
+    return SMLM_ERR_INVALID_ARGUMENT;   // (a row tile's queries may be read after another share has written its results)
   if (!aligned16(o) || !aligned16(q)) return SMLM_ERR_MISALIGNED;
   if (static_cast<long long>(total_q) * num_qo_heads > 0x7fffffffLL ||
       static_cast<long long>(total_pages) * page_size > 0x7fffffffLL ||
@@ -293,7 +293,8 @@ int smlm_b200_qk_norm_rope_bwd(void* dq, void* dk, void* dwq, void* dwk, const v
   if (T == 0) return SMLM_ERR_INVALID_ARGUMENT;   // a sum over no rows: the caller zeroes the weight gradients itself
   if (dq == nullptr || dk == nullptr || gq == nullptr || gk == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(gq) || !aligned16(gk)) return SMLM_ERR_MISALIGNED;
-  if (wq != nullptr) {
+  const bool dw = wq != nullptr && (dwq != nullptr || dwk != nullptr);
+  if (dw) {
     if (dwq == nullptr || dwk == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
     if (workspace == nullptr ||
         workspace_bytes < smlm_b200_qk_norm_rope_bwd_workspace_bytes(T, num_qo_heads, num_kv_heads))
@@ -301,13 +302,14 @@ int smlm_b200_qk_norm_rope_bwd(void* dq, void* dk, void* dwq, void* dwk, const v
     if (!aligned16(workspace)) return SMLM_ERR_MISALIGNED;
   }
   HeadNormArgs a = {};
-  a.positions = positions; a.T = T; a.pos64 = positions_64; a.eps = eps; a.partial = static_cast<float*>(workspace);
+  a.positions = positions; a.T = T; a.pos64 = positions_64; a.eps = eps; a.partial = dw ? static_cast<float*>(workspace) : nullptr;
   a.s[0].x = q; a.s[0].w = wq; a.s[0].g = gq; a.s[0].y = dq; a.s[0].stride = q_stride;
   a.s[1].x = k; a.s[1].w = wk; a.s[1].g = gk; a.s[1].y = dk; a.s[1].stride = k_stride;
   qk_bwd_streams(a, num_qo_heads, num_kv_heads);
   if (positions != nullptr) a.rot = rot_table(rope_theta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == SMLM_F16 ? launch_qk_bwd<__half>(a, dwq, dwk, st) : launch_qk_bwd<__nv_bfloat16>(a, dwq, dwk, st);
+  return dtype == SMLM_F16 ? launch_qk_bwd<__half>(a, dw ? dwq : nullptr, dwk, st)
+                           : launch_qk_bwd<__nv_bfloat16>(a, dw ? dwq : nullptr, dwk, st);
 }
 
 }  // extern "C"

@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kHnThreads, 2) qk_norm_rope_bwd_kernel(const _
     }
   }
   cp_async_wait<0>();
-  if (NORM) {
+  if (NORM && a.partial != nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float u, v;

@@ -124,7 +124,7 @@ __device__ __forceinline__ int ex_before(const ExArgs& a, const ExRequest& r, in
   const int first = r.len - r.n + (1 << lq) + kXtKeys - 1;   // row tile t: (first + t q) / 64, rounded down
   int sum;
   if (lq >= 6) {
-    sum = y * (first >> 6) + ((y * (y - 1)) >> 1 << (lq - 6));
+    sum = y * (first >> 6) + static_cast<int>((static_cast<unsigned>(y) * (y - 1)) >> 1 << (lq - 6));
   } else {                                            // the quotients go up by one every m = 64 / q row tiles
     const int lm = 6 - lq, f = first >> lq;
     auto steps = [&](unsigned i) {                    // sum of j >> lm for j < i, modulo 2^32: the difference is what counts

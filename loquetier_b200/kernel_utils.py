@@ -197,8 +197,8 @@ class qk_norm_rope(Function):
                 raise RuntimeError("positions must be int32 or int64")
         ctx.save_for_backward(q, k, q_weight, k_weight, positions)
         ctx.base, ctx.eps, ctx.strides = base, eps, strides
-        yq = torch.empty(q.shape, dtype=dtype, device=device)
-        yk = torch.empty(k.shape, dtype=dtype, device=device)
+        yq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        yk = torch.empty_like(k, memory_format=torch.contiguous_format)
         return ops.qk_norm_rope(yq, yk, q, k, q_weight, k_weight, positions, base, eps, strides)
 
     @staticmethod
@@ -207,11 +207,13 @@ class qk_norm_rope(Function):
         q, k, wq, wk, positions = ctx.saved_tensors
         # autograd's own nodes behind this one cannot be captured while an eager graph of the same leaves lives
         ops.refuse_capture(q, "the backward of qk_norm_rope")
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dwq, dwk = (None, None) if wq is None else (torch.empty_like(wq), torch.empty_like(wk))
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        dwq = dwk = None
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:   # weights that are not trained cost nothing
+            dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
         if q.size(0) == 0:
-            if wq is not None:
+            if dwq is not None:
                 dwq.zero_()
                 dwk.zero_()
         else:

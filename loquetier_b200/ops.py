@@ -452,10 +452,11 @@ def qk_norm_rope(yq, yk, q, k, wq, wk, positions, base: float, eps: float, strid
 
 def qk_norm_rope_bwd(dq, dk, dwq, dwk, gq, gk, q, k, wq, wk, positions, base: float, eps: float, strides=None,
                      workspace: Optional[torch.Tensor] = None):
-    """Gradients of ``qk_norm_rope``; gq, gk, dq and dk contiguous, dwq and dwk in the storage type (None without weights)."""
+    """Gradients of ``qk_norm_rope``; gq, gk, dq and dk contiguous, dwq and dwk in the storage type (None without weights or
+    where these are not trained)."""
     T, Nq, Nk = q.size(0), q.size(1), k.size(1)
     qs, ks = strides if strides is not None else _row_strides(q, k)
-    if workspace is None and wq is not None:
+    if workspace is None and dwq is not None:
         workspace = torch.empty(lib.smlm_b200_qk_norm_rope_bwd_workspace_bytes(T, Nq, Nk), dtype=torch.uint8, device=q.device)
     with on_device(q):
         check(lib.smlm_b200_qk_norm_rope_bwd(dq.data_ptr(), dk.data_ptr(), _p(dwq), _p(dwk), gq.data_ptr(), gk.data_ptr(),

@@ -122,6 +122,21 @@ def test_gradients_of_broadcast_and_transposed_outputs():
         assert (a.double() - b).abs().max() <= 4 * R.unit(torch.float16) * 8 * b.abs().max()
 
 
+@pytest.mark.parametrize("T", [1, 77])
+def test_weights_that_are_not_trained(T):
+    """Their gradients are not formed; the others are the same bits.  One of them alone may be trained."""
+    from loquetier_b200.kernel_utils import qk_norm_rope
+    q, k, _, wq, wk, gq, gk = _inputs(8, T, 8, 2, torch.bfloat16)
+    pos = torch.arange(T, device=DEV)
+    x = [t.detach().clone().requires_grad_() for t in (q, k)]
+    w = [t.detach().clone().requires_grad_() for t in (wq, wk)]
+    want = torch.autograd.grad(qk_norm_rope.apply(*x, *w, pos, BASE, EPS), x + w, (gq, gk))
+    got = torch.autograd.grad(qk_norm_rope.apply(*x, wq.detach(), wk.detach(), pos, BASE, EPS), x, (gq, gk))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = torch.autograd.grad(qk_norm_rope.apply(*x, wq.detach(), w[1], pos, BASE, EPS), x + w[1:], (gq, gk))
+    assert all(torch.equal(a, b) for a, b in zip(got, want[:2] + want[3:]))
+
+
 def test_backward_under_capture_is_refused():
     from loquetier_b200.kernel_utils import qk_norm_rope
     q, k, _, wq, wk, gq, gk = _inputs(7, 5, 4, 2, torch.bfloat16)

@@ -154,13 +154,14 @@ def test_c_abi_refusals():
     assert ws > 0 and L.smlm_b200_batch_extend_workspace_bytes(0, 8, 64, 16, 32, 8) == 0
     assert L.smlm_b200_batch_extend_workspace_bytes(1, 4, 2, 16, 300, 300) == 0     # a CTA per kv head: nothing is cut
 
-    def ext(o=256, wsp=256, bytes_=ws, rows=8, pages=64, nq=32, hd=128, layer=0, P=16, theta=10000.0, dt=1, batch=2):
+    def ext(o=512, wsp=256, bytes_=ws, rows=8, pages=64, nq=32, hd=128, layer=0, P=16, theta=10000.0, dt=1, batch=2):
         return L.smlm_b200_batch_extend(o, 256, 256, 256, 256, 256, wsp, bytes_, None, batch, rows, pages, nq, 8, hd, 1, layer,
                                         P, theta, dt, None)
 
     assert ext(dt=7) == 2 and ext(hd=64) == 3 and ext(P=128) == 3 and ext(P=12) == 3 and ext(nq=40) == 3 and ext(nq=36) == 3
     assert ext(layer=1) == 1 and ext(theta=0.0) == 1 and ext(rows=-1) == 1 and ext(o=None) == 1
     assert ext(o=264) == 4 and ext(wsp=264) == 4
+    assert ext(o=256) == 1   # in place
     assert ext(wsp=None) == 5 and ext(bytes_=ws - 1) == 5
     assert ext(rows=1 << 28) == 1 and ext(pages=1 << 28) == 1
     assert ext(batch=0) == 0 and ext(rows=0) == 0
@@ -186,6 +187,7 @@ def test_c_abi_refusals():
                                             32, 8, 128, 0, 1e4, 1e-6, 1, None)
 
     assert bwd(dq=None) == 1 and bwd(dwq=None) == 1 and bwd(T=0) == 1 and bwd(gq=264) == 4
+    assert bwd(dwq=None, wsp=None) == 1   # one gradient of the two
     assert bwd(wsp=None) == 5 and bwd(bytes_=need - 1) == 5 and bwd(wsp=264) == 4
 
     def app(yq=256, v=256, wq=256, vs=1024, ind=256, batch=2, T=5, P=16, layer=0):
