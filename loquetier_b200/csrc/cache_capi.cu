@@ -47,8 +47,8 @@ struct ExPlan {
 //   4 and 8  87 / 95 / 101    32  91 / 99 / 103    40  155 / 97 / 110    64  153 / 101 / 114    80  214 / 167 / 116
 // Keys rotated once in front (three more passes over them) or by every row tile that meets them, us, in place / in front, 32 / 8
 // heads, by rows per request:
-//   1 request on 16 k keys    256  67 / 69      384  81 / 77      512  95 / 85      1024  153 / 122    4096  489 / 333
-//   8 requests on 4 k keys    256  103 / 103    384  134 / 126    512  163 / 142    1024  282 / 230    4096  1052 / 798
+//   1 request on 16 k keys    128  50 / 56    256  69 / 69      320  81 / 73      512  97 / 83      1024  156 / 118    4096  490 / 308
+//   8 requests on 4 k keys    128  73 / 87    256  106 / 103    320  136 / 124    512  165 / 141    1024  288 / 226    4096  1070 / 767
 ExPlan extend_plan(int batch, int total_q, int total_pages, int page_size, int num_kv_heads, int group) {
   ExPlan p;
   const long long all_rows = static_cast<long long>(total_q) * group;

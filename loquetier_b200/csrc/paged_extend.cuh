@@ -14,7 +14,7 @@
 // follow from the lengths alone: the same batch gives the same result.
 //
 //   S[128, 64]   = Q . K_tile^T    tcgen05.mma, both operands K-major in shared memory, two accumulators in tensor memory
-//   P            = exp2(S - m)     a row is a tensor-memory lane, two threads per row
+//   P            = exp2(S - m)     a row is a tensor-memory lane, two threads per row (one where the keys are rotated in front)
 //   O[128, 128] += P . V_tile      A = P in tensor memory, B = V MN-major as the cache stores it
 //
 // The products and the softmax are those of the prefill kernel (paged_prefill.cuh).  What differs is where the tiles come
@@ -308,7 +308,9 @@ struct Xt {
   static constexpr int kKStages = 3, kVStages = QT == 4 ? 2 : 3;   // of the rings
   static constexpr int kSegs = QT == 1 ? 16 : 4;
   static constexpr int kRotWarps = DENSE ? 0 : 4;
-  static constexpr int kThreads = 32 * (2 * QT + kRotWarps + 4);
+  static constexpr int kHalves = DENSE ? 1 : 2;         // threads of a row
+  static constexpr int kSoft = 32 * QT * kHalves;       // softmax threads
+  static constexpr int kThreads = kSoft + 32 * (kRotWarps + 4);
   static constexpr int kQPanel = kRows * 128;           // Q: two 64-dim panels of [rows][128 B]
   static constexpr int kKOff = 2 * kQPanel;
   static constexpr int kVOff = kKOff + kKStages * kXtTileBytes;
@@ -399,6 +401,59 @@ __device__ __noinline__ void add_nonfinite(const ExArgs& a, const ExSeg& s, int 
     }
   }
 }
+// A run's queries, rotated and scaled by log2(e) / sqrt(d), as the A operand, K-major, where a thread has a row: a warp fetches its
+// 32 rows and rotates them in place.  Short loops, out of line: code that a warp comes to once per run waits for its
+// instructions (unrolled, with the rows in registers, this took 8000 cycles the first time and 1200 the second).  Eight prompts
+// of 512 tokens: 110 us instead of 118, of 1024: 230 instead of 259.  Where two threads share a row, and registers are
+// scarce, the same costs more in the loop over the keys than it gives: 229 us instead of 204 for 16 requests of 20 to 120 new
+// tokens, 32 heads.
+template <typename T>
+__device__ __noinline__ void bring_queries(const ExArgs& a, const ExSeg& s, uint32_t qs, int panel, int kvh, int wq) {
+  const int lg = a.lg, gmask = (1 << lg) - 1, row0 = s.row0 + wq * 32, nrows = s.nrows - wq * 32;
+  const int lane = threadIdx.x & 31;
+  qs += wq * 32 * 128;
+  const T* q = static_cast<const T*>(a.q);
+  const int Nq = a.num_kv_heads << lg;
+#pragma unroll 1
+  for (int i = lane; i < 32 * 16; i += 32) {
+    const int r = i >> 4, at = row0 + r, c = i & 7;   // a row's chunks of 16 bytes; eight to a panel
+    const T* src = q + (static_cast<size_t>(s.qo0 + (at >> lg)) * Nq + (kvh << lg) + (at & gmask)) * kPdDim + (i & 15) * 8;
+    cp_async16(qs + r * 128 + ((c ^ (r & 7)) << 4) + (i & 8 ? panel : 0), r < nrows ? src : q, r < nrows);
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+  __syncwarp();
+  // a thread turns eight dimensions and their partners of rows one after the other: the heads of a query share the sines
+  const int c = lane & 7;
+  float sn[8], cs[8];
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const int r = (lane >> 3) * 8 + i;
+    if ((i & gmask) == 0) {
+      const float scale = 1.4426950408889634f * rsqrtf(static_cast<float>(kPdDim));
+      const float pos = static_cast<float>(s.pos0 + ((row0 + r) >> lg));
+      const float *hi = rot_at(a.rot.hi) + c * 8, *lo = rot_at(a.rot.lo) + c * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        rot_sincos(pos, hi[k], lo[k], &sn[k], &cs[k]);
+        sn[k] *= scale;
+        cs[k] *= scale;
+      }
+    }
+    const uint32_t at = qs + r * 128 + ((c ^ (r & 7)) << 4);
+    uint32_t own[4], par[4];
+    lds128(at, own);
+    lds128(at + panel, par);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = unpack2<T>(own[k]), y = unpack2<T>(par[k]);
+      own[k] = pack2<T>(x.x * cs[2 * k] - y.x * sn[2 * k], x.y * cs[2 * k + 1] - y.y * sn[2 * k + 1]);
+      par[k] = pack2<T>(y.x * cs[2 * k] + x.x * sn[2 * k], y.y * cs[2 * k + 1] + x.y * sn[2 * k + 1]);
+    }
+    sts128(at, own);
+    sts128(at + panel, par);
+  }
+}
 // an entry of the page table, zero where there is none to read; without a branch, so that nothing waits for it here
 __device__ __forceinline__ uint64_t load_if(const void* const* at, bool yes) {
   uint64_t v;
@@ -411,6 +466,7 @@ __device__ __forceinline__ uint64_t load_if(const void* const* at, bool yes) {
 template <typename T, int QT, bool DENSE>
 __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_extend_kernel(const __grid_constant__ ExArgs a) {
   using X = Xt<QT, DENSE>;
+  constexpr int H = X::kHalves;
   constexpr int ROWS = X::kRows, NK = X::kKStages, NV = X::kVStages, ROTATORS = 32 * X::kRotWarps;
   extern __shared__ __align__(1024) unsigned char xt_smem[];
   const int tid = threadIdx.x, lane = tid & 31;
@@ -453,8 +509,8 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(xt_smem + (tmem_slot - sbase));
   // roles: softmax warps w < 8 with w mod 4 < QT; of the others, in the order of their numbers, the rotators, a loader of K,
   // one of V, the issuers of S and of O
-  const bool softmax = warp < 8 && (warp & 3) < QT;
-  const int other = warp - (warp < 4 ? min(warp, QT) : warp < 8 ? QT + min(warp - 4, QT) : 2 * QT);
+  const bool softmax = warp < 4 * H && (warp & 3) < QT;
+  const int other = warp - (warp < 4 ? min(warp, QT) : H == 2 && warp < 8 ? QT + min(warp - 4, QT) : H * QT);
   const int role = softmax ? -1 : max(0, other - X::kRotWarps + 1);   // 0 rotator, 1 K, 2 V, 3 S, 4 O
 
   ex_layout<ROWS, X::kThreads>(a, sc.begin, per, mine, a.cuts == nullptr ? nullptr : a.cuts + blockIdx.x, sc);
@@ -472,10 +528,10 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i * 8, 1);
-      mbar_init(p_full + i * 8, 64 * QT);
+      mbar_init(p_full + i * 8, X::kSoft);
       mbar_init(o_done + i * 8, 1);   // also: the S buffer, where P lives, is free
     }
-    mbar_init(q_full, 64 * QT);
+    mbar_init(q_full, X::kSoft);
     fence_mbar_init();
   }
   if (role == 3) {
@@ -694,10 +750,13 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
         }
       }
     } else {
-      // ---------------- softmax warps: thread = (row, half of the columns) ----------------
-      // Warps w and w + 4 (w < QT) hold the same 32 rows: the first takes columns 0-31 of a tile of S and 0-63 of O, the
-      // second the rest.  The two threads of a row agree on its maximum through tensor memory, as in the prefill kernel.
-      const int half = warp >> 2;
+      // ---------------- softmax warps: thread = (row, half of the columns), or a row ----------------
+      // H = 2: warps w and w + 4 (w < QT) hold the same 32 rows, the first takes columns 0-31 of a tile of S and 0-63 of O, the
+      // second the rest, and the two threads of a row agree on its maximum through tensor memory, as in the prefill kernel.
+      // H = 1: a thread has the row, and nothing is exchanged: with four warps in place of eight, and 128 registers a thread where
+      // nobody rotates, 230 us instead of 245 for 4 requests of 400 to 512 new tokens on 4 k to 12 k keys.  Beside rotators, with 80
+      // registers, 249 instead of 208 for 16 requests of 20 to 120 new tokens.
+      const int half = H == 2 ? warp >> 2 : 0;
       const int wq = warp & 3;
       const int row = wq * 32 + lane;
       const uint32_t my_tmem = tmem + (static_cast<uint32_t>(wq * 32) << 16);
@@ -708,11 +767,13 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
         // rows past the end behave like the last one
         const int my_pos = s.pos0 + (min(rr, s.row0 + s.nrows - 1) >> a.lg);
         // ---- the rotated, pre-scaled queries: A operand, K-major.  16 threads per row ----
-        {
+        if (H == 1) {
+          bring_queries<T>(a, sc.seg[seg], qs, X::kQPanel, kvh, wq);
+        } else {
           const int qt = (half * QT + wq) * 32 + lane;
           const int d0 = (qt & 15) * 4;
-          constexpr int PASS = 4 * QT;   // rows per pass
           const float qscale = 1.4426950408889634f * rsqrtf(static_cast<float>(kPdDim));   // log2(e) / sqrt(d)
+          constexpr int PASS = 4 * QT;   // rows per pass
           uint2 uo[8], up[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -746,9 +807,9 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
             asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(addr + X::kQPanel), "r"(pack2<T>(rp[0], rp[1])),
                          "r"(pack2<T>(rp[2], rp[3])) : "memory");
           }
-          fence_proxy_async();   // the products read Q through the async proxy
-          mbar_arrive(q_full);
         }
+        fence_proxy_async();   // the products read Q through the async proxy
+        mbar_arrive(q_full);
         if (wq * 32 >= s.nrows) {   // no row of the tile: hands on what the others make
           for (int j = 0; j < s.ntiles; ++j, ++g) {
             pf_wait_role(s_full + (g & 1) * 8, (g >> 1) & 1, a.err, dead);
@@ -765,29 +826,37 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
           tc_fence_after();
           const uint32_t my_s = my_tmem + sb * kXtKeys + half * kXtHalf;
           const int lim = my_pos - (s.tile0 + j) * kXtKeys - half * kXtHalf;   // columns above lim are later keys
-          uint32_t sv[32];
-          tc_ld32(my_s, sv);
+          uint32_t sv[3 - H][32];
+#pragma unroll
+          for (int h = 0; h < 3 - H; ++h) tc_ld32(my_s + h * kXtHalf, sv[h]);
           tc_wait_ld();
-          if (lim < 31) {
+          if (lim < 64 / H - 1) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i > lim) sv[i] = __float_as_uint(-INFINITY);
+            for (int i = 0; i < 64 / H; ++i)
+              if (i > lim) sv[i >> 5][i & 31] = __float_as_uint(-INFINITY);
           }
-          float ma = max3(__uint_as_float(sv[0]), __uint_as_float(sv[1]), __uint_as_float(sv[2]));
-          float mb = max3(__uint_as_float(sv[3]), __uint_as_float(sv[4]), __uint_as_float(sv[5]));
+          auto max_half = [](const uint32_t (&v)[32]) {
+            float ma = max3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
+            float mb = max3(__uint_as_float(v[3]), __uint_as_float(v[4]), __uint_as_float(v[5]));
 #pragma unroll
-          for (int i = 6; i < 30; i += 4) {
-            ma = max3(ma, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-            mb = max3(mb, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
+            for (int i = 6; i < 30; i += 4) {
+              ma = max3(ma, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              mb = max3(mb, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+            }
+            return fmaxf(max3(ma, __uint_as_float(v[30]), __uint_as_float(v[31])), mb);
+          };
+          float mx = max_half(sv[0]);
+          if (H == 1) {
+            mx = fmaxf(mx, max_half(sv[2 - H]));
+          } else {
+            // exchange with the other half's thread: own maximum into the first column of the own half
+            tc_st1(my_s, __float_as_uint(mx));
+            tc_wait_st();
+            tc_fence_before();
+            pair_barrier(wq);
+            tc_fence_after();
+            mx = fmaxf(mx, __uint_as_float(tc_ld1(my_tmem + sb * kXtKeys + (half ^ 1) * kXtHalf)));
           }
-          float mx = fmaxf(max3(ma, __uint_as_float(sv[30]), __uint_as_float(sv[31])), mb);
-          // exchange with the other half's thread: own maximum into the first column of the own half
-          tc_st1(my_s, __float_as_uint(mx));
-          tc_wait_st();
-          tc_fence_before();
-          pair_barrier(wq);
-          tc_fence_after();
-          mx = fmaxf(mx, __uint_as_float(tc_ld1(my_tmem + sb * kXtKeys + (half ^ 1) * kXtHalf)));
           float rescale = 1.0f;
           bool raise = false;
           if (mx > m_ref + kPfRaise || m_ref == -INFINITY) {   // (-inf + 8 = -inf: the first visible key always raises)
@@ -800,15 +869,22 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
           const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
           const uint64_t nm2 = pack_f32x2(nm, nm);
           uint64_t sum2 = pack_f32x2(0.f, 0.f);
-          uint32_t pw[kXtHalf / 2];
+          // P overwrites the upper half of the S columns that it was made of (the lower half keeps the exchanged maximum); the
+          // other thread of the row has read its own columns before the exchange
+          auto weights = [&](const uint32_t (&v)[32], int h) {
+            uint32_t pw[kXtHalf / 2];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float x0, x1;
-            unpack_f32x2(add_f32x2(pack_f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), nm2), x0, x1);
-            const float e0 = exp2f(x0), e1 = exp2f(x1);
-            sum2 = add_f32x2(sum2, pack_f32x2(e0, e1));
-            pw[i >> 1] = pack2<T>(e0, e1);
-          }
+            for (int i = 0; i < 32; i += 2) {
+              float x0, x1;
+              unpack_f32x2(add_f32x2(pack_f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), nm2), x0, x1);
+              const float e0 = exp2f(x0), e1 = exp2f(x1);
+              sum2 = add_f32x2(sum2, pack_f32x2(e0, e1));
+              pw[i >> 1] = pack2<T>(e0, e1);
+            }
+            tc_st16(my_s + h * kXtHalf + kXtHalf / 2, pw);
+          };
+          weights(sv[0], 0);
+          if (H == 1) weights(sv[2 - H], 1);
           l2 = add_f32x2(mul_f32x2(l2, pack_f32x2(rescale, rescale)), sum2);
           bool waited = j == 0;
           auto wait_prev = [&]() {   // P . V of the previous tile has completed: O is stable
@@ -821,7 +897,7 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
           if (j > 0 && __any_sync(0xffffffffu, raise)) {
             wait_prev();
 #pragma unroll 1
-            for (int q = 0; q < 2; ++q) {
+            for (int q = 0; q < 4 / H; ++q) {
               uint32_t ov[32];
               tc_ld32(o_tmem + q * 32, ov);
               tc_wait_ld();
@@ -831,9 +907,6 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
             }
             tc_wait_st();
           }
-          // P overwrites the upper half of the S columns this thread has read (the lower half keeps the exchanged
-          // maximum); the other thread of the row has read its own columns before the exchange
-          tc_st16(my_s + kXtHalf / 2, pw);
           tc_wait_st();
           tc_fence_before();
           mbar_arrive(p_full + sb * 8);
@@ -846,12 +919,15 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
         float la, lb;
         unpack_f32x2(l2, la, lb);
         const float l_mine = la + lb;
-        tc_st1(my_tmem + half * kXtHalf, __float_as_uint(l_mine));   // S buffer 0: the next product waits for this warp's queries
-        tc_wait_st();
-        tc_fence_before();
-        pair_barrier(wq);
-        tc_fence_after();
-        const float l_run = l_mine + __uint_as_float(tc_ld1(my_tmem + (half ^ 1) * kXtHalf));
+        float l_run = l_mine;
+        if (H == 2) {
+          tc_st1(my_tmem + half * kXtHalf, __float_as_uint(l_mine));   // S buffer 0: the next product waits for this warp's queries
+          tc_wait_st();
+          tc_fence_before();
+          pair_barrier(wq);
+          tc_fence_after();
+          l_run = l_mine + __uint_as_float(tc_ld1(my_tmem + (half ^ 1) * kXtHalf));
+        }
         const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;   // no keys: zeros; a NaN stays one
         T* orow = static_cast<T*>(a.o) + (static_cast<size_t>(s.qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim;
         float* rec = a.partial + (((static_cast<size_t>(share) * 2 + max(s.part, 0)) * a.num_kv_heads + kvh) * ROWS + row) * kPdRec;
@@ -861,7 +937,7 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
           rec[1] = l_run;
         }
 #pragma unroll 1
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < 4 / H; ++q) {
           uint32_t ov[32];
           tc_ld32(o_tmem + q * 32, ov);
           tc_wait_ld();
@@ -881,8 +957,10 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
             }
           }
         }
-        if (write && (sc.bad_v >> seg & 1))
-          add_nonfinite<T>(a, sc.seg[seg], kvh, half, my_pos, s.part >= 0 ? nullptr : orow + half * 64, rec + 4 + half * 64);
+        if (write && (sc.bad_v >> seg & 1)) {
+          for (int h = half; h < half + 3 - H; ++h)
+            add_nonfinite<T>(a, sc.seg[seg], kvh, h, my_pos, s.part >= 0 ? nullptr : orow + h * 64, rec + 4 + h * 64);
+        }
         tc_fence_before();   // the next row tile's products overwrite O after this warp has handed on a P
       }
     }

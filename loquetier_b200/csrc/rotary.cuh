@@ -7,9 +7,16 @@ namespace smlm {
 // The 64 frequencies in half-turns per position, base^(-2 i / 128) / pi, each as the sum of two floats: a product with
 // a position is then good to 2^-40 half-turns or so, where one float is off by several thousandths of a turn from
 // position 10^5 on - more than the rounding of a 16-bit result.
-struct RotTable {
+struct alignas(16) RotTable {
   float hi[64], lo[64];
 };
+
+// A place of the table that a launch carries among its arguments (__grid_constant__), for ordinary loads: lanes that index the
+// constant bank at places of their own are served one after another, some 30 cycles each.
+__device__ __forceinline__ const float* rot_at(const float* p) {
+  asm volatile("" : "+l"(p));
+  return p;
+}
 
 // cos and sin of pi * pos * (hi + lo) for positions below 2^24 in absolute value
 __device__ __forceinline__ void rot_sincos(float pos, float hi, float lo, float* s, float* c) {
@@ -23,9 +30,10 @@ __device__ __forceinline__ void rot_sincos(float pos, float hi, float lo, float*
 
 // the table into shared memory, [hi | lo]; every thread of the CTA takes part, a barrier follows at the caller
 __device__ __forceinline__ void load_rot_table(const RotTable& rot, float* freq) {
+  const float *hi = rot_at(rot.hi), *lo = rot_at(rot.lo);
   for (int i = threadIdx.x; i < 64; i += blockDim.x) {
-    freq[i] = rot.hi[i];
-    freq[64 + i] = rot.lo[i];
+    freq[i] = hi[i];
+    freq[64 + i] = lo[i];
   }
 }
 
