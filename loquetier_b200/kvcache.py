@@ -578,14 +578,14 @@ def batch_extend(q: torch.Tensor, qo_indptr: torch.Tensor, kv: BatchedKvCache, b
     last position.  Returns the attention output in the shape of ``q``; rows of no request are not written."""
     _chk_cuda_contig(q, "q", 3)
     _chk_cuda_contig(qo_indptr, "qo_indptr", 1)
+    pool = kv.pool
     if qo_indptr.dtype != torch.int32 or qo_indptr.numel() != kv.last_page_offset.numel() + 1:
         raise RuntimeError(f"qo_indptr must hold {kv.last_page_offset.numel() + 1} int32 values")
-    if q.dtype != kv.pool.dtype or q.size(2) != kv.pool.head_dim:
-        raise RuntimeError(f"q must be {kv.pool.dtype} with heads of {kv.pool.head_dim} like the cache")
+    if q.dtype != pool.dtype or q.size(2) != pool.head_dim:
+        raise RuntimeError(f"q must be {pool.dtype} with heads of {pool.head_dim} like the cache")
     _chk_same_device(q, qo_indptr=qo_indptr, kv=kv.ptrs)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    return batch_extend_into(o, q, qo_indptr, kv.ptrs, kv.indptr, kv.last_page_offset, kv.pool.num_layers, layer_idx,
-                             kv.pool.num_heads, base, kv.pool.page_len)
+    return batch_extend_into(torch.empty_like(q), q, qo_indptr, kv.ptrs, kv.indptr, kv.last_page_offset, pool.num_layers,
+                             layer_idx, pool.num_heads, base, pool.page_len)
 
 
 def norm_append_kv(kv: BatchedKvCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
@@ -599,18 +599,19 @@ def norm_append_kv(kv: BatchedKvCache, q: torch.Tensor, k: torch.Tensor, v: torc
     projection (rows any multiple of 8 elements apart, heads contiguous); ``q_weight`` and ``k_weight`` ``[head_dim]``.
     ``seqlen_indptr`` (int32, on the device): request b's tokens, as for ``init_kv``; None: one token per request, as for
     ``append_kv``.  Queries of rows of no request are not written."""
-    D = kv.pool.head_dim
+    pool = kv.pool
+    D, dtype = pool.head_dim, pool.dtype
     strides = [row_stride(t, name, D) for t, name in ((q, "q"), (k, "k"), (v, "v"))]
     for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         _chk_cuda_contig(t, name, 1)
         if t.numel() != D:
             raise RuntimeError(f"{name} must hold {D} values")
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (q_weight, "q_weight"), (k_weight, "k_weight")):
-        if t.dtype != kv.pool.dtype:
-            raise RuntimeError(f"{name} must be {kv.pool.dtype} like the cache")
+        if t.dtype != dtype:
+            raise RuntimeError(f"{name} must be {dtype} like the cache")
     batch, tokens = int(kv.last_page_offset.numel()), int(q.size(0))
-    if k.shape != v.shape or k.size(0) != tokens or k.size(1) != kv.pool.num_heads:
-        raise RuntimeError(f"k and v must be [{tokens}, {kv.pool.num_heads}, {D}]")
+    if k.shape != v.shape or k.size(0) != tokens or k.size(1) != pool.num_heads:
+        raise RuntimeError(f"k and v must be [{tokens}, {pool.num_heads}, {D}]")
     if seqlen_indptr is not None:
         _chk_cuda_contig(seqlen_indptr, "seqlen_indptr", 1)
         if seqlen_indptr.dtype != torch.int32 or seqlen_indptr.numel() != batch + 1:
@@ -619,7 +620,7 @@ def norm_append_kv(kv: BatchedKvCache, q: torch.Tensor, k: torch.Tensor, v: torc
         raise RuntimeError(f"without seqlen_indptr there must be one token per request. {tokens} vs {batch}")
     _chk_same_device(q, k=k, v=v, q_weight=q_weight, k_weight=k_weight, seqlen_indptr=seqlen_indptr, kv=kv.ptrs,
                      status_word=status_word)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     with on_device(q):
         check(lib.smlm_b200_norm_append_kv(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), q_weight.data_ptr(),
                                            k_weight.data_ptr(), kv.ptrs.data_ptr(), kv.indptr.data_ptr(),
@@ -627,6 +628,6 @@ def norm_append_kv(kv: BatchedKvCache, q: torch.Tensor, k: torch.Tensor, v: torc
                                            None if seqlen_indptr is None else seqlen_indptr.data_ptr(),
                                            None if status_word is None else status_word.data_ptr(), *strides, batch, tokens,
                                            int(kv.ptrs.numel()), int(q.size(1)), int(k.size(1)), D,
-                                           int(kv.pool.num_layers), int(layer_idx), int(kv.pool.page_len), float(eps),
+                                           int(pool.num_layers), int(layer_idx), int(pool.page_len), float(eps),
                                            _dtype_code(q), _stream(q)), "smlm_b200_norm_append_kv")
     return out

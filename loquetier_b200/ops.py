@@ -95,9 +95,12 @@ def row_stride(t: torch.Tensor, name: str, head_dim: int) -> int:
         raise RuntimeError(f"{name} must be a CUDA tensor")
     if t.dim() != 3 or t.size(2) != head_dim:
         raise RuntimeError(f"{name} must be [rows, heads, {head_dim}]")
-    if t.stride(2) != 1 or (t.size(1) > 1 and t.stride(1) != head_dim):
+    if t.is_contiguous():
+        return t.size(1) * head_dim
+    row, head, one = t.stride()
+    if one != 1 or (t.size(1) > 1 and head != head_dim):
         raise RuntimeError(f"the heads of a row of {name} must be contiguous")
-    return int(t.stride(0)) if t.size(0) > 1 else int(t.size(1)) * head_dim
+    return row if t.size(0) > 1 else t.size(1) * head_dim
 
 
 class Plan:
