@@ -37,8 +37,13 @@
 //
 // What bounds it (32 / 8 heads, B200).  32 requests, 512..4096 keys, 4 to 8 new tokens (285 MB, 44 us at the copy rate), 82 us a
 // pass: the launch 76, of which 6 are the search for the share and cold instructions, 5 the first tile, and the loop runs at
-// about the rate the pages arrive; the merge 5.  One request, 65 k keys, 17 tokens (269 MB): 85 us.  With 128 rows per tile the
-// loop is bound by issue slots (52 % used): of about 3400 warp instructions per tile, 1500 rotate, 1600 are the softmax's.
+// about the rate the pages arrive; the merge 5.  One request, 65 k keys, 17 tokens (269 MB): 84 us.  16 requests of 20 to 120
+// tokens, 32 heads (695 MB): 204.  With the rotation, the softmax and most of the products taken out, the copies and the
+// hand-offs between the roles alone take 73, 73 and 151 us (5.4 TB/s behind the start and in front of the merge), the hand-offs
+// without copies 45, 43 and 94: what is left to gain lies in the start, not in the arithmetic, but for tiles of 128 rows, where
+// rotation, softmax and products each lengthen a tile's way through the rings by 10 to 25 us.  Copies started early, into L2, gain
+// nothing.  4 requests of 400 to 512 tokens on 4 k to 12 k keys, 32 / 8 heads (160 GFLOP, 98 us): 226, of which the keys' rotation
+// in front 20, the merge 12; the tensor pipe is active 47 %, between hand-offs of P and S.
 // History on the first: one CTA per (row tile, range of keys) 146 us (CTAs of unequal length); even shares 100; roles whose
 // registers fit (spills in the loaders' loop) 94; copies and rotation in warps of their own 91; descriptors formed by one
 // addition, one barrier fewer, waits that sleep 84; key tiles counted exactly 82.  Waits that spin cost 5-15 % (they take
