@@ -137,6 +137,30 @@ def test_weights_that_are_not_trained(T):
     assert all(torch.equal(a, b) for a, b in zip(got, want[:2] + want[3:]))
 
 
+def test_offsets_past_32_bits():
+    """2^31 elements and more: the last rows are the bits that a call of their own gives, in both directions."""
+    from loquetier_b200.kernel_utils import qk_norm_rope
+    T, Nq, Nk, n = (1 << 31) // (64 * 128) + 5, 64, 1, 9
+    q = torch.empty((T, Nq, 128), dtype=torch.bfloat16, device=DEV)
+    k = torch.empty((T, Nk, 128), dtype=torch.bfloat16, device=DEV)
+    gq = torch.empty_like(q)
+    small = _inputs(9, n, Nq, Nk, torch.bfloat16)
+    for big, part in ((q, small[0]), (k, small[1]), (gq, small[5])):
+        big.normal_()
+        big[-n:] = part
+    gk = torch.ones_like(k)
+    pos = torch.arange(T, device=DEV)
+    wq, wk = small[3], small[4]
+    args = [q.requires_grad_(), k.requires_grad_()]
+    y = qk_norm_rope.apply(*args, wq, wk, pos, BASE, EPS)
+    tail = [t.detach()[-n:].clone().requires_grad_() for t in args]
+    ty = qk_norm_rope.apply(*tail, wq, wk, pos[-n:].contiguous(), BASE, EPS)
+    assert all(torch.equal(a[-n:], b) for a, b in zip(y, ty))
+    got = torch.autograd.grad(y, args, (gq, gk))
+    want = torch.autograd.grad(ty, tail, (gq[-n:].contiguous(), gk[-n:].contiguous()))
+    assert all(torch.equal(a[-n:], b) for a, b in zip(got, want))
+
+
 def test_backward_under_capture_is_refused():
     from loquetier_b200.kernel_utils import qk_norm_rope
     q, k, _, wq, wk, gq, gk = _inputs(7, 5, 4, 2, torch.bfloat16)
