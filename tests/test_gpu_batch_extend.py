@@ -98,7 +98,7 @@ def test_far_positions_lose_nothing():
 
 
 @pytest.mark.parametrize("requests,most,heads", [(300, 4, (2, 4)), (700, 3, (1, 8)), (3000, 2, (1, 1)), (700, 12, (1, 4)),
-                                                  (400, 30, (2, 4))])
+                                                  (400, 30, (2, 4)), (300, 90, (1, 8))])
 def test_uneven_batch_of_many_requests(requests, most, heads):
     """More requests than a CTA looks at together and more row tiles in a share than are laid out at a time; many without
     a new token, one far longer than the rest."""
