@@ -494,17 +494,6 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
     return;
   }
   const int kvh = blockIdx.x % a.num_kv_heads, share = blockIdx.x / a.num_kv_heads;
-  ExMine mine;
-  const int per = ex_share<ROWS, X::kThreads>(a, blockIdx.x == 0, mine, sc);
-  if (tid == 0) {
-    const long long begin = static_cast<long long>(share) * per;
-    sc.begin = static_cast<int>(min(begin, 0x7fffffffLL));
-    sc.end = static_cast<int>(min(begin + per, 0x7fffffffLL));
-  }
-  __syncthreads();
-  const int gmask = (1 << a.lg) - 1;
-  const int Nq = a.num_kv_heads << a.lg, P = a.page_size;
-
   const uint32_t qs = sbase, ks0 = sbase + X::kKOff, vs0 = sbase + X::kVOff, bars = sbase + X::kBarOff;
   const uint32_t k_raw = bars, k_full = k_raw + NK * 8, k_empty = k_full + NK * 8, v_full = k_empty + NK * 8, v_empty = v_full + NV * 8;
   // two each, used by alternate tiles: a softmax warp may be a tile ahead of another, and looks at the completion of a tile
@@ -517,9 +506,6 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
   const bool softmax = warp < 4 * H && (warp & 3) < QT;
   const int other = warp - (warp < 4 ? min(warp, QT) : H == 2 && warp < 8 ? QT + min(warp - 4, QT) : H * QT);
   const int role = softmax ? -1 : max(0, other - X::kRotWarps + 1);   // 0 rotator, 1 K, 2 V, 3 S, 4 O
-
-  ex_layout<ROWS, X::kThreads>(a, sc.begin, per, mine, a.cuts == nullptr ? nullptr : a.cuts + blockIdx.x, sc);
-  if (sc.count == 0) return;   // nothing left for this share (uniform over the CTA)
 
   if (tid == 0) {
     for (int i = 0; i < NK; ++i) {
@@ -543,10 +529,25 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
     tc_alloc(tmem_slot, kXtTmemCols);
     tc_relinquish();
   }
-  tc_fence_before();
+  tc_fence_before();   // (the search for the share has barriers enough, and hides what this takes)
+  ExMine mine;
+  const int per = ex_share<ROWS, X::kThreads>(a, blockIdx.x == 0, mine, sc);
+  if (tid == 0) {
+    const long long begin = static_cast<long long>(share) * per;
+    sc.begin = static_cast<int>(min(begin, 0x7fffffffLL));
+    sc.end = static_cast<int>(min(begin + per, 0x7fffffffLL));
+  }
   __syncthreads();
+  const int gmask = (1 << a.lg) - 1;
+  const int Nq = a.num_kv_heads << a.lg, P = a.page_size;
+
+  ex_layout<ROWS, X::kThreads>(a, sc.begin, per, mine, a.cuts == nullptr ? nullptr : a.cuts + blockIdx.x, sc);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot_ptr;
+  if (sc.count == 0) {   // nothing left for this share (uniform over the CTA)
+    if (role == 3) tc_dealloc(tmem, kXtTmemCols);
+    return;
+  }
   bool dead = false;
   int g = 0, gs = 0;   // tiles and row tiles so far, of the warp's role
 
