@@ -163,15 +163,21 @@ struct ExScratch {
   ExSeg seg[SEGS];              // runs of the share that are laid out at a time
 };
 
-// Running sums over the CTA's threads in their order: returns what the threads before this one hold, `all` the whole.
+// Running sums over the CTA's threads in their order: returns what the threads before this one hold, `all` the whole.  Where only
+// the first warp's threads hold anything (up to 32 requests) it does without the others, for whom `all` is nothing: whatever
+// follows from it is the first warp's as well.
 template <int NT, typename S>
-__device__ __forceinline__ long long ex_scan(long long v, long long& all, S& sc) {
+__device__ __forceinline__ long long ex_scan(long long v, long long& all, S& sc, bool one_warp) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long incl = v;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const long long up = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += up;
+  }
+  if (one_warp) {
+    all = __shfl_sync(0xffffffffu, incl, 31);
+    return incl - v;
   }
   __syncthreads();
   if (lane == 31) sc.sum[warp] = incl;
@@ -217,7 +223,7 @@ __device__ __forceinline__ ExMine ex_mine(const ExArgs& a, int b0, long long& be
     m.work = ex_work<ROWS>(a, m.r);
   }
   long long all;
-  const long long at = before + ex_scan<NT>(m.work, all, sc);
+  const long long at = before + ex_scan<NT>(m.work, all, sc, a.batch <= 32);
   before += all;
   m.at = static_cast<int>(min(at, 0x7fffffffLL));   // (more work than that is refused, see ex_share)
   return m;
@@ -271,7 +277,7 @@ __device__ __forceinline__ void ex_layout(const ExArgs& a, int w0, unsigned per,
       n = tile_at(to - 1) - first + 1;
     }
     long long all_segs;
-    int i = static_cast<int>(min(segs + ex_scan<NT>(n, all_segs, sc), static_cast<long long>(SEGS)));
+    int i = static_cast<int>(min(segs + ex_scan<NT>(n, all_segs, sc, a.batch <= 32), static_cast<long long>(SEGS)));
     for (int tile = first; tile < first + n && i < SEGS; ++tile, ++i) {
       const int start = ex_before<ROWS>(a, m.r, tile), nt = ex_before<ROWS>(a, m.r, tile + 1) - start;
       const int k0 = max(from, start) - start, k1 = min(to, start + nt) - start;
