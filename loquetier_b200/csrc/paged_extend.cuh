@@ -36,9 +36,9 @@
 // of the rings and half of the tensor cores' time again.  Scores, maxima, sums and parked states are fp32.
 //
 // What bounds it (32 / 8 heads, B200).  32 requests, 512..4096 keys, 4 to 8 new tokens (285 MB, 44 us at the copy rate), 82 us a
-// pass: the launch 76, of which 6 are the search for the share and cold instructions, 5 the first tile, and the loop runs at
-// about the rate the pages arrive; the merge 5.  One request, 65 k keys, 17 tokens (269 MB): 84 us.  16 requests of 20 to 120
-// tokens, 32 heads (695 MB): 204.  With the rotation, the softmax and most of the products taken out, the copies and the
+// pass: the launch 76, of which 5 are the search for the share and cold instructions, 5 the first tile, and the loop runs at
+// about the rate the pages arrive; the merge 5.  One request, 65 k keys, 17 tokens (269 MB): 81 us.  16 requests of 20 to 120
+// tokens, 32 heads (695 MB): 200 to 208.  With the rotation, the softmax and most of the products taken out, the copies and the
 // hand-offs between the roles alone take 73, 73 and 151 us (5.4 TB/s behind the start and in front of the merge), the hand-offs
 // without copies 45, 43 and 94: what is left to gain lies in the start, not in the arithmetic, but for tiles of 128 rows, where
 // rotation, softmax and products each lengthen a tile's way through the rings by 10 to 25 us.  Copies started early, into L2, gain
