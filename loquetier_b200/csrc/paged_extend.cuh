@@ -978,7 +978,7 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
     }
     if (sc.next >= sc.end) break;
     const int w0 = sc.next;
-    __syncthreads();   // everyone is done with this round's runs
+    __syncthreads();   // everyone is done with these runs
     long long before = 0;
     if (a.batch <= X::kThreads) mine = ex_mine<ROWS, X::kThreads>(a, 0, before, sc);
     ex_layout<ROWS, X::kThreads>(a, w0, 1u, mine, nullptr, sc);
