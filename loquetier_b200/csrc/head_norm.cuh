@@ -285,7 +285,9 @@ __global__ void __launch_bounds__(kHnThreads, 2) qk_norm_rope_bwd_kernel(const _
       }
       float u, v;
       unpack_f32x2(ss2, u, v);
-      const float s = rsqrtf(sum8(u + v) * (1.0f / kPdDim) + a.eps);
+      const float mean = sum8(u + v) * (1.0f / kPdDim) + a.eps;
+      // (lanes behind the last head hold zeros: without an epsilon their factor would be infinite, and their share of dw a NaN)
+      const float s = h < heads ? rsqrtf(mean) : 0.f;
       unpack_f32x2(dot2, u, v);
       const float coef = -sum8(u + v) * s * s * (1.0f / kPdDim);
       const uint64_t s2 = pack_f32x2(s, s), coef2 = pack_f32x2(coef, coef);
