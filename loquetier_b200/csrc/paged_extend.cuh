@@ -197,7 +197,8 @@ struct ExCut {
   int qo0, row0, nrows;   // as in ExSeg; no rows: the share starts a row tile, or holds no work
   int first, shares;      // the row tile's first share, and how many more it lies in: that many CTAs merge
   int part;               // where the first share has its state; the others have it at 0
-  int pad[2];
+  int pos0;               // as in ExSeg
+  int pad;
 };
 
 // keys that a row of row tile `tile` of the request sees
@@ -205,6 +206,12 @@ template <int ROWS>
 __device__ __forceinline__ int ex_visible(const ExArgs& a, const ExRequest& r, int tile) {
   const int last = min((r.n << a.lg), (tile + 1) * ROWS) - 1;
   return max(0, min(r.len, r.len - r.n + (last >> a.lg) + 1));
+}
+
+// What a row of weight sum l at position pos is multiplied by.  A row that sees no key is zeros; one that sees keys, but none whose
+// score is above -inf (products that leave fp32's range), has no answer, and a NaN says so.  A NaN stays one.
+__device__ __forceinline__ float row_scale(float l, int pos) {
+  return l != 0.f ? 1.0f / l : pos < 0 ? 0.f : __int_as_float(0x7fffffff);
 }
 
 // A thread's request of those that the CTA looks at together, its work and its place in the head's work.
@@ -300,7 +307,8 @@ __device__ __forceinline__ void ex_layout(const ExArgs& a, int w0, unsigned per,
         c.first = begin / per;
         c.shares = (begin + nt - 1) / per - c.first;
         c.part = begin == c.first * per ? 0 : 1;
-        c.pad[0] = c.pad[1] = 0;
+        c.pos0 = s.pos0;
+        c.pad = 0;
         *cut = c;
         wrote = true;
       }
@@ -940,7 +948,7 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
           tc_fence_after();
           l_run = l_mine + __uint_as_float(tc_ld1(my_tmem + (half ^ 1) * kXtHalf));
         }
-        const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;   // no keys: zeros; a NaN stays one
+        const float inv = row_scale(l_run, my_pos);
         T* orow = static_cast<T*>(a.o) + (static_cast<size_t>(s.qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim;
         float* rec = a.partial + (((static_cast<size_t>(share) * 2 + max(s.part, 0)) * a.num_kv_heads + kvh) * ROWS + row) * kPdRec;
         const bool write = row < s.nrows && !dead;
@@ -1070,7 +1078,7 @@ __global__ void __launch_bounds__(kXtMergeThreads) paged_extend_merge_kernel(con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int4* rec = reinterpret_cast<const int4*>(a.cuts + blockIdx.x + a.num_kv_heads);
   const int4 c0 = __ldcg(rec), c1 = __ldcg(rec + 1);
-  const int qo0 = c0.x, row0 = c0.y, nrows = c0.z, first = c0.w, shares = c1.x, part = c1.y;
+  const int qo0 = c0.x, row0 = c0.y, nrows = c0.z, first = c0.w, shares = c1.x, part = c1.y, pos0 = c1.z;
   const int gmask = (1 << a.lg) - 1, Nq = a.num_kv_heads << a.lg;
   const size_t share_step = static_cast<size_t>(2) * a.num_kv_heads * ROWS * kPdRec;
   if (nrows == 0) return;
@@ -1098,8 +1106,8 @@ __global__ void __launch_bounds__(kXtMergeThreads) paged_extend_merge_kernel(con
     }
   };
   auto write_row = [&](int row, float l, const float4& acc) {
-    const float inv = l == 0.f ? 0.f : 1.0f / l;   // no keys: zeros; a NaN stays one
     const int rr = row0 + row;
+    const float inv = row_scale(l, pos0 + (rr >> a.lg));
     T* op = static_cast<T*>(a.o) + (static_cast<size_t>(qo0 + (rr >> a.lg)) * Nq + (kvh << a.lg) + (rr & gmask)) * kPdDim;
     reinterpret_cast<uint2*>(op)[lane] = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
   };
