@@ -260,10 +260,7 @@ template <int ROWS, int NT, int SEGS>
 __device__ __forceinline__ void ex_layout(const ExArgs& a, int w0, unsigned per, const ExMine& m0, ExCut* cut,
                                           ExScratch<SEGS>& sc) {
   const int w_begin = sc.begin, w_end = sc.end;
-  if (threadIdx.x == 0) {
-    sc.next = w_end;
-    sc.bad_v = 0;
-  }
+  if (threadIdx.x == 0) sc.bad_v = 0;
   long long before = 0, segs = 0;
   bool wrote = false;
   for (int b0 = 0; b0 < a.batch && before < w_end && segs < SEGS; b0 += NT) {
@@ -317,7 +314,10 @@ __device__ __forceinline__ void ex_layout(const ExArgs& a, int w0, unsigned per,
   }
   if (cut != nullptr && !__syncthreads_or(wrote) && threadIdx.x == 0) cut->nrows = 0;
   __syncthreads();
-  if (threadIdx.x == 0) sc.count = static_cast<int>(min(segs, static_cast<long long>(SEGS)));
+  if (threadIdx.x == 0) {
+    sc.count = static_cast<int>(min(segs, static_cast<long long>(SEGS)));
+    if (segs < SEGS) sc.next = w_end;   // (otherwise whoever laid out the last run has stored it: one writer in either case)
+  }
   __syncthreads();
 }
 

@@ -1,8 +1,10 @@
 """``kvcache.batch_extend`` at the edges of its range."""
+import random
+
 import pytest
 import torch
 
-from test_gpu_batch_extend import DEV, LAYER, _batch, _run
+from test_gpu_batch_extend import DEV, LAYER, _batch, _check, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +28,13 @@ def test_scores_that_leave_the_range(new, length, group):
     first = max(0, at - (length - new))                  # the first query that sees it
     assert torch.isnan(o[:first]).all()
     assert torch.equal(o[first:new], dense[0][1][at].expand_as(o[first:new]))
+
+
+@pytest.mark.parametrize("requests,new,heads", [(20, 3, (296, 1)), (32, 5, (200, 4)), (31, 100, (64, 1)), (7, 700, (40, 1)),
+                                                (32, 300, (74, 1))])
+def test_few_requests_of_more_runs_than_are_laid_out_at_a_time(requests, new, heads):
+    """Many kv heads leave each of them few CTAs, so that a share holds more row tiles than one round (16, or 4 of 64 rows and
+    more).  Up to 32 requests are searched by one warp."""
+    r = random.Random(requests)
+    runs = [r.randint(max(1, new // 2), new) for _ in range(requests)]
+    _check(requests, [n + r.randint(0, 40) for n in runs], runs, *heads, 16, torch.bfloat16)
