@@ -179,8 +179,8 @@ int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, con
   if (group != 1 && group != 2 && group != 4 && group != 8) return SMLM_ERR_NO_KERNEL;
   if (batch_size == 0 || total_q == 0) return SMLM_OK;
   if (o == nullptr || q == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || last_page_offset == nullptr ||
-      (kv_ptrs == nullptr && total_pages > 0) || o == q)
-    return SMLM_ERR_INVALID_ARGUMENT;   // (a row tile's queries may be read after another share has written its results)
+      (kv_ptrs == nullptr && total_pages > 0))
+    return SMLM_ERR_INVALID_ARGUMENT;
   if (!aligned16(o) || !aligned16(q)) return SMLM_ERR_MISALIGNED;
   if (static_cast<long long>(total_q) * num_qo_heads > 0x7fffffffLL ||
       static_cast<long long>(total_pages) * page_size > 0x7fffffffLL ||
@@ -192,6 +192,10 @@ int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, con
     if (workspace == nullptr || workspace_bytes < p.bytes) return SMLM_ERR_WORKSPACE;
     if (!aligned16(workspace)) return SMLM_ERR_MISALIGNED;
   }
+  // (a row tile's queries may be read after another share has written its results)
+  const uintptr_t o_at = reinterpret_cast<uintptr_t>(o), q_at = reinterpret_cast<uintptr_t>(q);
+  const uintptr_t q_bytes = static_cast<uintptr_t>(total_q) * num_qo_heads * kPdDim * 2;
+  if (o_at - q_at < q_bytes || q_at - o_at < q_bytes) return SMLM_ERR_INVALID_ARGUMENT;
   ExArgs a;
   a.o = o; a.q = q; a.qo_indptr = qo_indptr; a.kv_ptrs = kv_ptrs; a.kv_indptr = kv_indptr;
   a.last_page_offset = last_page_offset; a.err = status_word;

@@ -38,3 +38,22 @@ def test_few_requests_of_more_runs_than_are_laid_out_at_a_time(requests, new, he
     r = random.Random(requests)
     runs = [r.randint(max(1, new // 2), new) for _ in range(requests)]
     _check(requests, [n + r.randint(0, 40) for n in runs], runs, *heads, 16, torch.bfloat16)
+
+
+def test_results_right_beside_the_queries():
+    """Results in front of the queries and behind them, in one allocation, without a byte between them; one byte group
+    less is refused."""
+    pool, args, starts, dense = _batch(60, [300, 50], [5, 3], 2, 4, 16, torch.bfloat16)
+    args["q"] = q = args["q"][:starts[-1]].contiguous()
+    want = _run(args)
+    n = q.numel()
+    from loquetier_b200 import kvcache
+    room = torch.zeros(3 * n, dtype=q.dtype, device=DEV)
+    args["q"] = room[n:2 * n].view(q.shape)
+    for first in (0, 2 * n):
+        args["q"].copy_(q)
+        o = kvcache.batch_extend_into(room[first:first + n].view(q.shape), **args)
+        assert torch.equal(o, want) and torch.equal(args["q"], q)
+    for first in (8, 2 * n - 8, n):
+        with pytest.raises(RuntimeError):
+            kvcache.batch_extend_into(room[first:first + n].view(q.shape), **args)
