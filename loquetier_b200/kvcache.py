@@ -234,14 +234,14 @@ class KvCache:
         if init_len < 0:
             raise ValueError("init_len must be non-negative")
         self._pool = pool
-        if init_len > 0:
-            npages = (init_len + pool.page_len - 1) // pool.page_len
-            self._pages = [pool.alloc_page() for _ in range(npages)]
-            self._seqlen = init_len
-        else:
-            self._pages = []
-            self._seqlen = 0
-        self._ptrs = GrowableTensor([t.data_ptr() for t in self._pages], dtype=torch.int64, device=pool.device)
+        self._pages = pool.alloc_pages((init_len + pool.page_len - 1) // pool.page_len)
+        self._seqlen = init_len
+        try:
+            self._ptrs = GrowableTensor([t.data_ptr() for t in self._pages], dtype=torch.int64, device=pool.device)
+        except BaseException:
+            for page in self._pages:
+                pool.free_page(page)
+            raise
 
     pool = property(lambda self: self._pool)
     seqlen = property(lambda self: self._seqlen)

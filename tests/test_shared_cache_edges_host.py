@@ -1,4 +1,6 @@
 """Host side of the operators around a shared cache: refusals and what a failure leaves behind.  No GPU."""
+import pytest
+import torch
 
 
 def test_results_that_overlap_the_queries_are_refused():
@@ -14,3 +16,34 @@ def test_results_that_overlap_the_queries_are_refused():
 
     for o in (q, q + 16, q - 16, q + 256, q + nbytes - 16, q - nbytes + 16):
         assert ext(o) == 1
+
+
+@pytest.mark.parametrize("fails", ["slab", "table"])
+def test_a_cache_that_cannot_be_made_keeps_no_pages(monkeypatch, fails):
+    """The memory ends at the third slab, or at the table of addresses: the pages taken so far are free again, and their slabs
+    can be given back."""
+    from loquetier_b200 import kvcache
+    pool = kvcache.KvPool(1, 1, 8, 4, torch.float32, "cpu", pages_per_slab=2)
+    kept = kvcache.KvCache(pool, 5)
+    real, slabs = torch.empty, []
+
+    def empty(*a, **kw):
+        slabs.append(1)
+        if len(slabs) == 3:
+            raise RuntimeError("out of memory")
+        return real(*a, **kw)
+
+    def table(*a, **kw):
+        raise RuntimeError("out of memory")
+
+    if fails == "slab":
+        monkeypatch.setattr(torch, "empty", empty)
+    else:
+        monkeypatch.setattr(kvcache, "GrowableTensor", table)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        kvcache.KvCache(pool, 30)
+    monkeypatch.undo()
+    assert pool.num_pages == 2 and [p.data_ptr() for p in pool.allocated_pages()] == [p.data_ptr() for p in kept.pages]
+    assert len(pool._free) == pool.num_slabs * 2 - 2
+    kept.release()
+    assert pool.compact([kept]) and pool.num_slabs == 0
