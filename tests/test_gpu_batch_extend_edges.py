@@ -4,7 +4,9 @@ import random
 import pytest
 import torch
 
-from test_gpu_batch_extend import DEV, LAYER, _batch, _check, _run
+import shared_cache_ref as R
+from extend_whole import check_whole
+from test_gpu_batch_extend import BASE, DEV, LAYER, _batch, _check, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +59,24 @@ def test_results_right_beside_the_queries():
     for first in (8, 2 * n - 8, n):
         with pytest.raises(RuntimeError):
             kvcache.batch_extend_into(room[first:first + n].view(q.shape), **args)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [(8, 4), (1, 8), (3, 1), (1, 1)])
+@pytest.mark.parametrize("new,length", [(1, 5003), (2, 5003), (7, 9001), (1, 20011), (17, 4099), (33, 2500), (130, 3333)])
+def test_long_caches_as_acheck_whole(dtype, heads, new, length):
+    """Few rows over many keys: values so small that the elementwise bounds would let a zero pass."""
+    pool, args, starts, dense = _batch(new, [length], [new], *heads, 16, dtype)
+    want, _ = R.extend(args["q"], starts, dense, BASE)
+    check_whole(_run(args)[:new], want[:new], dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 31])
+def test_small_batches_as_acheck_whole(dtype, rows):
+    lens, new = [rows + 350, 900, 700 + rows], [rows, 1, rows]
+    pool, args, starts, dense = _batch(rows, lens, new, 1, 1, 16, dtype)
+    want, _ = R.extend(args["q"], starts, dense, BASE)
+    o = _run(args)
+    for t0, t1 in zip(starts, starts[1:]):
+        check_whole(o[t0:t1], want[t0:t1], dtype)

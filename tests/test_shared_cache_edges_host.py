@@ -2,6 +2,9 @@
 import pytest
 import torch
 
+import shared_cache_ref as R
+from extend_whole import check_whole
+
 
 def test_results_that_overlap_the_queries_are_refused():
     """Any common byte, from either side, with everything else in order; refused before any CUDA call."""
@@ -47,3 +50,33 @@ def test_a_cache_that_cannot_be_made_keeps_no_pages(monkeypatch, fails):
     assert len(pool._free) == pool.num_slabs * 2 - 2
     kept.release()
     assert pool.compact([kept]) and pool.num_slabs == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [(8, 4), (1, 8), (3, 1), (1, 1)])
+@pytest.mark.parametrize("new,length", [(1, 5003), (2, 5003), (7, 9001)])
+def test_the_check_as_a_whole_rejects_what_is_lost(dtype, heads, new, length):
+    """For few rows over many keys the elementwise bounds let a zero pass; the check of the whole result does not, nor a
+    share of 4 tiles of 64 keys that is lost or counted twice.  Roundings pass."""
+    (N, G), cut = heads, slice(256, 512)
+    g = torch.Generator().manual_seed(new)
+    q = torch.randn((new, N * G, 128), generator=g).to(dtype)
+    K, V = (torch.randn((length, N, 128), generator=g).to(dtype) for _ in range(2))
+    want, _ = R.extend(q, [0, new], [(K, V)], 1e4)
+    check_whole(want.to(dtype), want, dtype)
+
+    def attend(weight):   # keys counted so often, in 64 bits
+        pos = torch.arange(length)
+        kr, qr = R.rotate(K.double(), pos, 1e4), R.rotate(q.double(), pos[-new:], 1e4)
+        s = torch.einsum("nhgd,lhd->nhgl", qr.unflatten(1, (N, G)), kr) / 128 ** 0.5
+        e = torch.exp(s) * weight * (pos[None] <= pos[-new:, None]).double()[:, None, None]
+        return torch.einsum("nhgl,lhd->nhgd", e / e.sum(-1, keepdim=True), V.double()).flatten(1, 2)
+
+    weight = torch.ones(length, dtype=torch.float64)
+    check_whole(attend(weight).to(dtype), want, dtype)
+    for wrong in (0.0, 2.0):
+        weight[cut] = wrong
+        with pytest.raises(AssertionError):
+            check_whole(attend(weight), want, dtype)
+    with pytest.raises(AssertionError):
+        check_whole(torch.zeros_like(want), want, dtype)
