@@ -360,8 +360,8 @@ int smlm_b200_rms_norm_bwd(void* dx, void* dw, const void* go, const void* x, co
  *   n = x * rsqrt(mean(x^2) + eps) * w            (wq and wk [head_dim]; both NULL: n = x)
  *   y = n rotated for positions[t], Llama convention with base rope_theta   (positions NULL: y = n)
  * in fp32, rounded once to the 16-bit `dtype`; yq and yk contiguous.  Weights, positions or both.  positions: int32, or int64
- * where positions_64 is set, below 2^24 in absolute value; the angles are formed to 2^-40 turns, so that far positions
- * lose nothing.  No workspace. */
+ * where positions_64 is set, below 2^24 in absolute value; angles are reduced to 2^-24 turns and sines and cosines good to
+ * 2^-20, so that far positions lose nothing.  No workspace. */
 int smlm_b200_qk_norm_rope(void* yq, void* yk, const void* q, const void* k, const void* wq, const void* wk,
                            const void* positions, long long q_stride, long long k_stride, int T, int num_qo_heads,
                            int num_kv_heads, int head_dim, int positions_64, double rope_theta, float eps, int dtype,

@@ -4,9 +4,10 @@
 
 namespace smlm {
 
-// The 64 frequencies in half-turns per position, base^(-2 i / 128) / pi, each as the sum of two floats: a product with
-// a position is then good to 2^-40 half-turns or so, where one float is off by several thousandths of a turn from
-// position 10^5 on - more than the rounding of a 16-bit result.
+// The 64 frequencies in half-turns per position, base^(-2 i / 128) / pi, each as the sum of two floats.  The pair is good to
+// 2^-51 of a half-turn per position, 2^-27 at position 2^24; what rot_sincos adds is the rounding of the reduced angle to one
+// float, 2^-24 half-turns.  One float alone is off by several thousandths of a turn from position 10^5 on - more than the
+// rounding of a 16-bit result.
 struct alignas(16) RotTable {
   float hi[64], lo[64];
 };
@@ -18,7 +19,8 @@ __device__ __forceinline__ const float* rot_at(const float* p) {
   return p;
 }
 
-// cos and sin of pi * pos * (hi + lo) for positions below 2^24 in absolute value
+// cos and sin of pi * pos * (hi + lo) for positions below 2^24 in absolute value; measured up to there, against 64 bits and more:
+// off by 2^-20.4 at most (the reduced angle's roundings to a float, and the fast sine)
 __device__ __forceinline__ void rot_sincos(float pos, float hi, float lo, float* s, float* c) {
   const float a = __fmul_rn(pos, hi);
   const float e = __fmaf_rn(pos, lo, __fmaf_rn(pos, hi, -a));   // what a lacks

@@ -1,4 +1,5 @@
 """``kvcache.batch_extend`` at the edges of its range."""
+import math
 import random
 
 import pytest
@@ -80,3 +81,62 @@ def test_small_batches_as_acheck_whole(dtype, rows):
     o = _run(args)
     for t0, t1 in zip(starts, starts[1:]):
         check_whole(o[t0:t1], want[t0:t1], dtype)
+
+
+@pytest.mark.parametrize("new", [3, 300])
+def test_near_the_last_position(new):
+    """A cache that ends 37 keys short of 2^24, its last 4096 keys the ones that count, at scores of 20 and some that hang
+    on the rotation: single-precision angles, off by half a radian there, give another result.  (One page of keys that score
+    zero and have no value stands in for all the pages in front: the table may name a page more than once.)
+
+    Every key is the rotation back of a vector u_j, every query that of t_i, so that the scores are t_i . u_j whatever the
+    position.  Bound as in ``shared_cache_ref.extend``, with 2^-13 in a pair's turn for the angles (sines good to 2^-19, 63
+    steps of a recurrence that adds them up)."""
+    P, L, near, dtype = 64, (1 << 24) - 37, 4096, torch.float16
+    assert L % P and near % P == 0
+    u = R.unit(dtype)
+    g = torch.Generator(device=DEV).manual_seed(new)
+    fast = torch.zeros(128, dtype=torch.float64, device=DEV)
+    fast[:8] = fast[64:72] = 1.0                           # the eight fastest pairs
+    ahead = -(-L // P) - near // P                         # pages in front
+    pos = torch.arange(ahead * P, L, device=DEV)
+    rand = lambda *s: torch.randn(s, generator=g, device=DEV, dtype=torch.float64)
+    t = fast * (1 + 0.3 * rand(new, 1, 128))
+    key = fast * 14.0 * (1 + 0.2 * rand(pos.numel(), 1, 128))   # scores of 14 * 16 / sqrt(128) or so
+    value = rand(pos.numel(), 1, 128).to(dtype)
+    q = R.rotate(t, -pos[-new:], BASE).to(dtype)
+    k = R.rotate(key, -pos, BASE).to(dtype)
+    pool = torch.zeros((1 + near // P, 1, 2, 1, P, 128), dtype=dtype, device=DEV)
+    pad = torch.zeros(near, 1, 128, dtype=dtype, device=DEV)
+    for i, x in enumerate((k, value)):
+        pad[:pos.numel()] = x
+        pool[1:, 0, i, 0] = pad.view(-1, P, 128)
+    table = [0] * ahead + list(range(1, 1 + near // P))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    ptrs = pool.data_ptr() + torch.tensor(table, dtype=torch.int64, device=DEV) * (pool[0].numel() * pool.element_size())
+    o = _run(dict(q=q, qo_indptr=i32([0, new]), kv_ptrs=ptrs, kv_indptr=i32([0, len(table)]),
+                  last_page_offset=i32([(L - 1) % P + 1]), num_layers=1, layer_idx=0, num_kv_heads=1, base=BASE, page_size=P))
+
+    def attend(rot):
+        kr, qr = rot(k, pos)[:, 0], rot(q, pos[-new:])[:, 0]
+        seen = pos[None] <= pos[-new:, None]
+        e = torch.where(seen, torch.exp(qr @ kr.t() / math.sqrt(128)), 0.0)
+        p = e / (e.sum(1, keepdim=True) + ahead * P)
+        size = (qr.abs() @ kr.abs().t() / math.sqrt(128)).amax(1, keepdim=True)
+        return p @ value[:, 0].double(), p @ value[:, 0].double().abs(), size
+
+    def single(x, at):   # the angles as products of floats
+        freq = (BASE ** (-torch.arange(64, dtype=torch.float64, device=DEV) / 64)).float()
+        ang = (at.float()[:, None] * freq).double()
+        c, s, a, b = ang.cos()[:, None], ang.sin()[:, None], x[..., :64].double(), x[..., 64:].double()
+        return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+    want, mass, size = attend(lambda x, at: R.rotate(x.double(), at, BASE))
+    d = (2 * u * (1 + u) + 2.0 ** -13) * size
+    bound = u * want.abs() + (u + torch.expm1(2 * d) + 2.0 ** -15) * mass
+    err, other = (o[:, 0].double() - want).abs(), (attend(single)[0] - want).abs()
+    assert (err <= bound).all(), f"{int((err > bound).sum())} past, worst {(err / bound).max()}"
+    # as a whole: a score's roundings are 0.6 u of its size at most in the root mean square
+    limit = ((0.6 * u + 2.0 ** -13) * size.max() + 1.3 * u).item()
+    assert (err.norm() / want.norm()).item() <= limit
+    assert (other > bound).any() and (other.norm() / want.norm()).item() > 2 * limit   # what the test is for
