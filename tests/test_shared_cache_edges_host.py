@@ -80,3 +80,19 @@ def test_the_check_as_a_whole_rejects_what_is_lost(dtype, heads, new, length):
             check_whole(attend(weight), want, dtype)
     with pytest.raises(AssertionError):
         check_whole(torch.zeros_like(want), want, dtype)
+
+
+def test_the_backward_asks_first_whether_a_capture_runs(monkeypatch):
+    """Without a GPU: nothing of the saved tensors is used before the refusal."""
+    from types import SimpleNamespace
+
+    from loquetier_b200 import ops
+    from loquetier_b200.kernel_utils import qk_norm_rope
+
+    def refuse(t, what):
+        raise RuntimeError(f"{what} cannot be captured")
+
+    monkeypatch.setattr(ops, "refuse_capture", refuse)
+    ctx = SimpleNamespace(saved_tensors=(None,) * 5)   # anything done with them would raise something else
+    with pytest.raises(RuntimeError, match="the backward of qk_norm_rope cannot be captured"):
+        qk_norm_rope.backward(ctx, None, None)
