@@ -89,7 +89,11 @@ int dispatch_extend(const ExArgs& a, const ExPlan& p, cudaStream_t stream) {
   }
 }
 
-// warps that share a token's heads: few tokens are spread over the machine, four heads per warp at least
+// Warps that share a token's heads: few tokens are spread over the machine (2368 warps, two CTAs per SM), four heads per warp at
+// least.  bf16, us of one launch among others, by this rule / one warp per token / a warp per four heads always:
+//   32 / 8 heads, forward    1 token  1.8 / 3.4 / 1.8    181  3.3 / 5.0 / 3.3    600  5.3 / 6.1 / 6.2    2048  10.5 / 8.9 / 16.1
+//                 8192  31 / 31 / 62        backward    64  4.5 / 7.8 / 4.6    600  9.7 / 9.1 / 9.7    8192  50 / 51 / 58
+//   32 / 32 heads, into the cache    64  3.2 / 9.5 / 3.2    600  6.6 / 12.2 / 7.5    2048  20.1 / 20.0 / 22.3
 inline int head_splits(int T, int heads) {
   const int want = (8 * kNumSMs * 2 + T - 1) / std::max(T, 1);
   return std::max(1, std::min(want, (heads + 3) / 4));
@@ -137,8 +141,7 @@ int launch_qk_bwd(const HeadNormArgs& a, void* dwq, void* dwk, cudaStream_t stre
 
 // the checks that both directions share; rows that are strided have to keep the 16-byte alignment of every head
 int qk_check(const void* q, const void* k, const void* wq, const void* wk, const void* positions, long long q_stride,
-             long long k_stride, int T, int Nq, int Nk, int head_dim, int positions_64, double rope_theta, int dtype) {
-  (void)positions_64;
+             long long k_stride, int T, int Nq, int Nk, int head_dim, double rope_theta, int dtype) {
   if (T < 0 || Nq <= 0 || Nk <= 0 || (wq == nullptr) != (wk == nullptr) || (wq == nullptr && positions == nullptr) ||
       (positions != nullptr && !(rope_theta > 0.0)))
     return SMLM_ERR_INVALID_ARGUMENT;
@@ -237,8 +240,8 @@ int smlm_b200_norm_append_kv(void* yq, const void* q, const void* k, const void*
   if (batch_size < 0 || total_tokens < 0 || total_pages < 0 || num_layers <= 0 || layer_idx < 0 ||
       layer_idx >= num_layers || (seqlen_indptr == nullptr && total_tokens != batch_size) || wq == nullptr || wk == nullptr)
     return SMLM_ERR_INVALID_ARGUMENT;
-  const int rc = qk_check(q, k, wq, wk, nullptr, q_stride, k_stride, total_tokens, num_qo_heads, num_kv_heads, head_dim, 0,
-                          1.0, dtype);
+  const int rc = qk_check(q, k, wq, wk, nullptr, q_stride, k_stride, total_tokens, num_qo_heads, num_kv_heads, head_dim, 1.0,
+                          dtype);
   if (rc != SMLM_OK) return rc;
   if (!kv_shape_ok(head_dim, page_size)) return SMLM_ERR_NO_KERNEL;
   if (batch_size == 0 || total_tokens == 0) return SMLM_OK;
@@ -264,7 +267,7 @@ int smlm_b200_qk_norm_rope(void* yq, void* yk, const void* q, const void* k, con
                            int num_kv_heads, int head_dim, int positions_64, double rope_theta, float eps, int dtype,
                            void* stream) {
   const int rc = qk_check(q, k, wq, wk, positions, q_stride, k_stride, T, num_qo_heads, num_kv_heads, head_dim,
-                          positions_64, rope_theta, dtype);
+                          rope_theta, dtype);
   if (rc != SMLM_OK || T == 0) return rc;
   if (yq == nullptr || yk == nullptr) return SMLM_ERR_INVALID_ARGUMENT;
   if (!aligned16(yq) || !aligned16(yk)) return SMLM_ERR_MISALIGNED;
@@ -292,7 +295,7 @@ int smlm_b200_qk_norm_rope_bwd(void* dq, void* dk, void* dwq, void* dwk, const v
                                int num_kv_heads, int head_dim, int positions_64, double rope_theta, float eps, int dtype,
                                void* stream) {
   const int rc = qk_check(q, k, wq, wk, positions, q_stride, k_stride, T, num_qo_heads, num_kv_heads, head_dim,
-                          positions_64, rope_theta, dtype);
+                          rope_theta, dtype);
   if (rc != SMLM_OK) return rc;
   if (T == 0) return SMLM_ERR_INVALID_ARGUMENT;   // a sum over no rows: the caller zeroes the weight gradients itself
   if (dq == nullptr || dk == nullptr || gq == nullptr || gk == nullptr) return SMLM_ERR_INVALID_ARGUMENT;

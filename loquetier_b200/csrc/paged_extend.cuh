@@ -43,8 +43,9 @@
 // hand-offs between the roles alone take 73, 73 and 151 us (5.4 TB/s behind the start and in front of the merge), the hand-offs
 // without copies 45, 43 and 94: what is left to gain lies in the start, not in the arithmetic, but for tiles of 128 rows, where
 // rotation, softmax and products each lengthen a tile's way through the rings by 10 to 25 us.  Copies started early, into L2, gain
-// nothing.  4 requests of 400 to 512 tokens on 4 k to 12 k keys, 32 / 8 heads (160 GFLOP, 98 us): 226, of which the keys' rotation
-// in front 20, the merge 12; the tensor pipe is active 47 %, between hand-offs of P and S.
+// nothing.  4 requests of 400 to 512 tokens on 4 k to 12 k keys, 32 / 8 heads (160 GFLOP, 98 us): 241 to 247 where the inputs change
+// from pass to pass, 219 on the same ones; by the launch 20 for the keys' rotation in front, 197, 12 for the merge.  The tensor
+// pipe is active 47 %, between hand-offs of P and S.
 // History on the first: one CTA per (row tile, range of keys) 146 us (CTAs of unequal length); even shares 100; roles whose
 // registers fit (spills in the loaders' loop) 94; copies and rotation in warps of their own 91; descriptors formed by one
 // addition, one barrier fewer, waits that sleep 84; key tiles counted exactly 82.  Waits that spin cost 5-15 % (they take
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(Xt<QT, DENSE>::kThreads, kXtCtasPerSm) paged_e
     const int count = sc.count;
     if (!DENSE && role == 0) {
       // ---------------- rotators: thread = (chunk c of 8 dims and its partner, every STEP-th key) ----------------
-      constexpr int STEP = DENSE ? 32 : ROTATORS / 8, KPT = kXtKeys / STEP;   // keys of a thread per tile
+      constexpr int STEP = 32 * Xt<QT>::kRotWarps / 8, KPT = kXtKeys / STEP;   // KPT: keys of a thread per tile
       const int rt = other * 32 + lane, c = rt & 7, kr = rt >> 3;
       const ulonglong2* my_turn = reinterpret_cast<const ulonglong2*>(turn) + c * 4;
       uint64_t cc[4] = {}, ss[4] = {};   // cosines and sines of key kr + STEP i, two frequencies each
@@ -1052,9 +1053,6 @@ __global__ void __launch_bounds__(128) extend_rotate_kernel(const __grid_constan
   }
 }
 
-// Merges the states of the row tiles that are cut, in the order of the keys.  grid: ((shares - 1) * Nkv, kXtMergeSplit); a
-// CTA stands for the cut at the start of a share and serves some of the rows of the tile that it goes through, a warp a row
-// at a time, a lane four dimensions.
 // adds one softmax state to another; an empty one (no weight) carries no information
 __device__ __forceinline__ void add_state(float m1, float l1, const float4& o1, float& m, float& l, float4& acc) {
   if (l1 == 0.f) return;
@@ -1070,6 +1068,9 @@ __device__ __forceinline__ void add_state(float m1, float l1, const float4& o1, 
 constexpr int kXtMergeThreads = 256;
 constexpr int kXtMergeSplit = 2;   // (four to eight times as many CTAs of fewer rows measured the same or slower)
 
+// Merges the states of the row tiles that are cut, in the order of the keys.  grid: ((shares - 1) * Nkv, kXtMergeSplit); a
+// CTA stands for the cut at the start of a share and serves some of the rows of the tile that it goes through, a warp a row
+// at a time, a lane four dimensions.
 template <typename T, int QT>
 __global__ void __launch_bounds__(kXtMergeThreads) paged_extend_merge_kernel(const __grid_constant__ ExArgs a) {
   constexpr int ROWS = Xt<QT>::kRows, WARPS = kXtMergeThreads / 32;
