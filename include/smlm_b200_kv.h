@@ -117,8 +117,9 @@ size_t smlm_b200_batch_extend_workspace_bytes(int batch_size, int total_q, int t
  * and keys `dtype`: an fp16 pair (dimensions i, i + 64) of a key longer than 65504 may turn into an infinity.  For positions
  * below 2^24 angles are reduced to 2^-24 turns; the queries' sines and cosines are good to 2^-20, the keys', formed by a recurrence
  * of up to 63 steps, to 2^-15.  A key or value that is not finite reaches the tokens that see it and no others.  o must not
- * overlap q (refused).  Status word: bit 1 also where a request has more queries than keys; value 8: a bounded wait inside the
- * kernel gave up (the output is then not valid). */
+ * overlap q (refused).  A batch whose row tiles (32 to 128 rows, one more per request) times key tiles (64 keys, one more per
+ * request), both over the whole batch, reach 2^31 is refused as an invalid argument: cut it.  Status word: bit 1 also where a
+ * request has more queries than keys; value 8: a bounded wait inside the kernel gave up (the output is then not valid). */
 int smlm_b200_batch_extend(void* o, const void* q, const int32_t* qo_indptr, const void* const* kv_ptrs,
                            const int32_t* kv_indptr, const int32_t* last_page_offset, void* workspace,
                            size_t workspace_bytes, int* status_word, int batch_size, int total_q, int total_pages,

@@ -41,9 +41,9 @@
 // about the rate the pages arrive; the merge 5.  One request, 65 k keys, 17 tokens (269 MB): 81 us.  16 requests of 20 to 120
 // tokens, 32 heads (695 MB): 200 to 208.  With the rotation, the softmax and most of the products taken out, the copies and the
 // hand-offs between the roles alone take 73, 73 and 151 us (5.4 TB/s behind the start and in front of the merge), the hand-offs
-// without copies 45, 43 and 94: what is left to gain lies in the start, not in the arithmetic, but for tiles of 128 rows, where
-// rotation, softmax and products each lengthen a tile's way through the rings by 10 to 25 us.  Copies started early, into L2, gain
-// nothing.  4 requests of 400 to 512 tokens on 4 k to 12 k keys, 32 / 8 heads (160 GFLOP, 98 us): 241 to 247 where the inputs change
+// without copies 45, 43 and 94: what is left to gain in this form lies in the copies and the start, not in the arithmetic, but
+// for tiles of 128 rows, where rotation, softmax and products each lengthen a tile's way through the rings by 10 to 25 us.  Copies
+// started early, into L2, gain nothing.  4 requests of 400 to 512 tokens on 4 k to 12 k keys, 32 / 8 heads (160 GFLOP, 98 us): 241 to 247 where the inputs change
 // from pass to pass, 219 on the same ones; by the launch 20 for the keys' rotation in front, 197, 12 for the merge.  The tensor
 // pipe is active 47 %, between hand-offs of P and S.
 // History on the first: one CTA per (row tile, range of keys) 146 us (CTAs of unequal length); even shares 100; roles whose

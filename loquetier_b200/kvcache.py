@@ -575,7 +575,11 @@ def batch_extend(q: torch.Tensor, qo_indptr: torch.Tensor, kv: BatchedKvCache, b
     already holds their keys and values (drafted tokens to verify, a conversation's next turn, a prompt taken in
     pieces).  ``q`` ``[sum(new tokens), num_heads, head_dim]`` and the keys in ``kv`` are NOT position encoded; request b owns
     rows ``qo_indptr[b] .. qo_indptr[b + 1]`` (int32, on the device; it may own none), its last one stands at the cache's
-    last position.  Returns the attention output in the shape of ``q``; rows of no request are not written."""
+    last position.  Returns the attention output in the shape of ``q``; rows of no request are not written.
+
+    1, 2, 4 or 8 query heads per kv head, ``q`` contiguous.  Whole prompts, and many requests with 64 new tokens or more on short
+    caches, are faster through ``batch_prefill``.  Batches whose row tiles times key tiles (of up to 128 rows and 64 keys, over the
+    whole batch) reach 2^31 are refused."""
     _chk_cuda_contig(q, "q", 3)
     _chk_cuda_contig(qo_indptr, "qo_indptr", 1)
     pool = kv.pool
